@@ -26,7 +26,7 @@ CENSUS = ["binary", "bcast", "unary", "row_op", "gemm", "gemv_f32", "gemv_bf16",
           "gemv_q4", "attn_decode", "rope", "rmsnorm", "rmsnorm_res", "swiglu", "argmax",
           "kv_append", "kv_fill", "split_heads", "merge_heads", "gemm_bf16_nt", "attn_prefill",
           "convert", "quantize_q4", "mix_step", "window_attn", "linear_attn", "polynorm", "embed", "residual",
-          "ssm", "latent_attn", "act"]
+          "ssm", "latent_attn", "act", "quantize_mx", "gemv_mxfp4", "gemm_mxfp4"]
 
 # name -> (restype, argtypes): exactly the declarations of include/tensorlib_hip.h
 SIGNATURES = {
@@ -147,6 +147,15 @@ SIGNATURES = {
     "tlhip_rms_rows": (cint, [P, i64, P, P, i64, i64, i64, i64, f32, i64]),
     "tlhip_geglu_rows": (cint, [P, P, P, i64, i64]),
     "tlhip_embed_scaled": (cint, [P, i64, P, P, i64, i64, i64, i64, f32]),
+    "tlhip_quantize_mxfp4": (cint, [P, cint, P, P, i64, i64]),
+    "tlhip_quantize_mxfp8": (cint, [P, P, P, i64, i64]),
+    "tlhip_dequantize_mxfp4": (cint, [P, P, P, cint, i64, i64]),
+    "tlhip_dequantize_mxfp8": (cint, [P, P, P, cint, i64, i64]),
+    "tlhip_rmsnorm_res_mxfp8": (cint, [P, P, i64, P, P, P, P, i64, f32, i64]),
+    "tlhip_gemv_mxfp4": (cint, [P, P, P, P, i64, i64]),
+    "tlhip_gemm_mxfp4_nt": (cint, [P, P, P, P, P, i64, i64, i64]),
+    "tlhip_gemm_mxfp4_nt_parts": (cint, [P, P, P, P, P, i64, i64, i64, i64, P]),
+    "tlhip_gemm_mxfp4_nt_swiglu": (cint, [P, P, P, P, P, P, i64, i64, i64]),
     "tlhip_ssm_state_bytes": (i64, [i64, i64, i64]),
     "tlhip_ssm_conv_bytes": (i64, [i64, i64, i64, i64, i64]),
     "tlhip_ssm_step": (cint, [P, P, P, i64, P]),
@@ -561,6 +570,39 @@ class TlHip:
         total = rows if total_rows is None else total_rows
         self._chk(self.c.tlhip_quantize_q4(src.ptr, src_type, q4buf.ptr + row_base * K // 2,
                                            q4buf.ptr + total * K // 2 + row_base * (K // 32) * 4, rows, K, group))
+
+    # microscaled formats: elements and scales in buffers of their own
+    def quantize_mxfp4(self, src, src_type, codes, scales, rows, K):
+        self._chk(self.c.tlhip_quantize_mxfp4(src.ptr, src_type, codes.ptr, scales.ptr, rows, K))
+
+    def quantize_mxfp8(self, x, codes, scales, rows, K):
+        self._chk(self.c.tlhip_quantize_mxfp8(x.ptr, codes.ptr, scales.ptr, rows, K))
+
+    def dequantize_mxfp4(self, codes, scales, dst, dst_type, rows, K):
+        self._chk(self.c.tlhip_dequantize_mxfp4(codes.ptr, scales.ptr, dst.ptr, dst_type, rows, K))
+
+    def dequantize_mxfp8(self, codes, scales, dst, dst_type, rows, K):
+        self._chk(self.c.tlhip_dequantize_mxfp8(codes.ptr, scales.ptr, dst.ptr, dst_type, rows, K))
+
+    def rmsnorm_res_mxfp8(self, x, parts, n_parts, w, xout, codes, scales, n, eps, rows=1):
+        self._chk(self.c.tlhip_rmsnorm_res_mxfp8(x.ptr, parts.ptr if parts is not None else None, n_parts, w.ptr,
+                                                 xout.ptr if xout is not None else None, codes.ptr, scales.ptr, n, eps, rows))
+
+    def gemv_mxfp4(self, a, codes, scales, y, N, K):
+        self._chk(self.c.tlhip_gemv_mxfp4(a.ptr, codes.ptr, scales.ptr, y.ptr, N, K))
+
+    def gemm_mxfp4_nt(self, acodes, ascales, codes, scales, out, M, N, K):
+        self._chk(self.c.tlhip_gemm_mxfp4_nt(acodes.ptr, ascales.ptr, codes.ptr, scales.ptr, out.ptr, M, N, K))
+
+    def gemm_mxfp4_nt_parts(self, acodes, ascales, codes, scales, parts, M, N, K):
+        n = C.c_int(0)
+        self._chk(self.c.tlhip_gemm_mxfp4_nt_parts(acodes.ptr, ascales.ptr, codes.ptr, scales.ptr, parts.ptr, parts.nbytes, M, N, K,
+                                                   C.byref(n)))
+        return n.value
+
+    def gemm_mxfp4_nt_swiglu(self, acodes, ascales, codes, scales, act_codes, act_scales, M, ff, K):
+        self._chk(self.c.tlhip_gemm_mxfp4_nt_swiglu(acodes.ptr, ascales.ptr, codes.ptr, scales.ptr, act_codes.ptr, act_scales.ptr,
+                                                    M, ff, K))
 
     def embed_gather_f16(self, table, d_token, out, hidden, vocab):
         self._chk(self.c.tlhip_embed_gather_f16(table.ptr, d_token.ptr, out.ptr, hidden, vocab))

@@ -101,7 +101,8 @@ typedef enum {
   TLHIP_C_ARGMAX, TLHIP_C_KV_APPEND, TLHIP_C_KV_FILL, TLHIP_C_SPLIT_HEADS,
   TLHIP_C_MERGE_HEADS, TLHIP_C_GEMM_BF16_NT, TLHIP_C_ATTN_PREFILL, TLHIP_C_CONVERT,
   TLHIP_C_QUANTIZE_Q4, TLHIP_C_MIX_STEP, TLHIP_C_WINDOW_ATTN, TLHIP_C_LINEAR_ATTN, TLHIP_C_POLYNORM,
-  TLHIP_C_EMBED, TLHIP_C_RESIDUAL, TLHIP_C_SSM, TLHIP_C_LATENT_ATTN, TLHIP_C_ACT, TLHIP_C_COUNT
+  TLHIP_C_EMBED, TLHIP_C_RESIDUAL, TLHIP_C_SSM, TLHIP_C_LATENT_ATTN, TLHIP_C_ACT,
+  TLHIP_C_QUANTIZE_MX, TLHIP_C_GEMV_MXFP4, TLHIP_C_GEMM_MXFP4, TLHIP_C_COUNT
 } tlhip_census_id;
 int tlhip_census(uint64_t* counts, int n);  /* copies min(n, TLHIP_C_COUNT) counters */
 int tlhip_census_reset(void);
@@ -627,6 +628,40 @@ typedef struct {
 int64_t tlhip_latent_cache_bytes(int64_t capacity, int64_t kv_rank, int64_t rot_dim, int64_t planes, int values);
 int tlhip_latent_attn_run(const void* u, int64_t ldu, const void* q, int64_t ldq, void* y, int64_t ldy,
                           const tlhip_latent_attn* a, int64_t T, int64_t pos0, const void* d_pos);
+
+/* ---- microscaled formats (no reference counterpart) -------------------------------------------------
+ * MXFP4 weights and MXFP8 rows of activations, the formats that the scaled matrix instructions of gfx950 multiply. A row is cut
+ * into blocks of 32 elements; a block's scale byte s stands for 2^(s - 127) (255: the whole block is NaN), its elements are
+ *   MXFP4: e2m1 codes, magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6; [rows][K/2] bytes, even k in the low nibble;
+ *   MXFP8: e4m3 bytes, magnitudes up to 448 (0x7f, 0xff: NaN); [rows][K] bytes;
+ * scales [rows][K/32] bytes in both. Rows are dense and K is a multiple of 32, so rows of two matrices of the same K can be stacked.
+ * Rounding a block: s = floor(log2(largest magnitude)) + 127 - 2 (MXFP4) or - 8 (MXFP8), at least 0; every element is the value
+ * over 2^(s - 127), rounded to nearest, ties to even, magnitudes beyond the type's largest becoming that. A block that holds
+ * an infinity or a NaN gets the scale 255 and elements 0. Elements must be 16-byte aligned, scales need no alignment. */
+/* rows of TLHIP_T_F32, _F16 or _BF16 as a model file holds them -> MXFP4 */
+int tlhip_quantize_mxfp4(const void* src, int src_type, void* codes, void* scales, int64_t rows, int64_t K);
+/* f32 rows -> MXFP8 */
+int tlhip_quantize_mxfp8(const void* x, void* codes, void* scales, int64_t rows, int64_t K);
+/* the values as f32 or bf16 (exact in both, but that bf16 rounds what lies below 2^-126) */
+int tlhip_dequantize_mxfp4(const void* codes, const void* scales, void* dst, int dst_type, int64_t rows, int64_t K);
+int tlhip_dequantize_mxfp8(const void* codes, const void* scales, void* dst, int dst_type, int64_t rows, int64_t K);
+/* xout = x + (parts[0] + ... + parts[S-1]) in f32, ascending, parts [S][rows][n] (S = 0: none, parts may be NULL);
+ * h = xout / sqrt(mean(xout^2) + eps) * w in 64 bits, rounded to f32, then to MXFP8. xout may be NULL, or x; not the parts.
+ * n up to 32768, S up to 64. A row's bytes do not depend on how many rows there are. */
+int tlhip_rmsnorm_res_mxfp8(const void* x, const void* parts, int64_t S, const void* w, void* xout, void* codes, void* scales,
+                            int64_t n, float eps, int64_t rows);
+/* y[n] = sum_k a[k] W[n][k], a f32, W MXFP4 [N][K], f32 sums: the decode product. */
+int tlhip_gemv_mxfp4(const void* a, const void* codes, const void* scales, void* y, int64_t N, int64_t K);
+/* C[M][N] f32 = A . W^T, A MXFP8 [M][K], W MXFP4 [N][K]: products of elements are exact, sums are f32. _parts as
+ * tlhip_gemm_bf16_nt_parts. */
+int tlhip_gemm_mxfp4_nt(const void* acodes, const void* ascales, const void* codes, const void* scales, void* C, int64_t M, int64_t N,
+                        int64_t K);
+int tlhip_gemm_mxfp4_nt_parts(const void* acodes, const void* ascales, const void* codes, const void* scales, void* parts,
+                              int64_t parts_bytes, int64_t M, int64_t N, int64_t K, int* n_parts);
+/* W = [gate rows | up rows], [2 ff][K]: the gated activation swiglu(A . gate^T, A . up^T) as MXFP8 rows of ff (a multiple of
+ * 32), what the down projection reads; the products are never written. */
+int tlhip_gemm_mxfp4_nt_swiglu(const void* acodes, const void* ascales, const void* codes, const void* scales, void* act_codes,
+                               void* act_scales, int64_t M, int64_t ff, int64_t K);
 
 /* Upper bound on the K splits of the [K,N] GEMVs (tlhip_gemv_f32 / tlhip_gemv_bf16); 1 = no
  * split, 0 = the built-in choice. The reference's diagnostic knob set_no_splitk (cuda.h:193-197,

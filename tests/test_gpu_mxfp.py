@@ -1,0 +1,416 @@
+"""Microscaled formats on the GPU: rounding and reading back bit for bit, the norm whose result is MXFP8, and the products over MXFP4
+weights against 64 bits.
+
+Tolerance of the products: elements multiply exactly (4 by 2 significant bits), so only sums round. An element's product meets at
+most 128 additions inside a matrix instruction, one for each of the K/128 instructions, and one for each of up to 64 parts, terms or
+wavefronts whose sums are joined: |error| <= (128 + K/128 + 64) 2^-24 sum |a w|. The f32 row of the decode product
+is carried to 2^-38 of its block's largest, which is below one of those roundings per element for a spread of up to 2^14.
+"""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import mx_oracle as mx
+
+pytestmark = pytest.mark.gpu
+EPS = 1e-6
+
+
+def rng(*key):
+    return np.random.default_rng(list(key))
+
+
+def activations(r, rows, k):
+    """Rows with some columns an order larger, some blocks of zeros, some of small numbers."""
+    x = r.standard_normal((rows, k)) * np.where(r.random(k) < 0.02, 13, 1)
+    b = x.reshape(rows, -1, 32)
+    b[r.random(b.shape[:2]) < 0.02] = 0
+    b[r.random(b.shape[:2]) < 0.02] *= 1e-4
+    return x.astype(np.float32)
+
+
+def weight(r, n, k):
+    codes, scales = mx.quantize((r.standard_normal((n, k)) * 0.02).astype(np.float32), True)
+    return codes, scales
+
+
+def rows8(r, m, k):
+    return mx.quantize(activations(r, m, k), False)
+
+
+def guarded(lib, nbytes):
+    """Room for nbytes with 256 bytes of 0xa5 behind them."""
+    b = lib.empty_bytes(nbytes + 256)
+    b.upload(np.full(nbytes + 256, 0xa5, np.uint8))
+    return b
+
+
+def taken(b, nbytes, dtype, shape):
+    raw = b.numpy(np.uint8)
+    assert (raw[nbytes:] == 0xa5).all(), "wrote behind the result"
+    return raw[:nbytes].view(dtype).reshape(shape)
+
+
+def half_types(x, t):
+    if t == "f32":
+        return x
+    if t == "f16":
+        return x.astype(np.float16)
+    u = x.astype(np.float32).view(np.uint32)
+    return ((u + 0x7fff + (u >> 16 & 1)) >> 16).astype(np.uint16)
+
+
+def widened(x, t):
+    return x.astype(np.float32) if t != "bf16" else (x.astype(np.uint32) << 16).view(np.float32)
+
+
+def hard_values(r, rows, k):
+    """What rounding can go wrong at: borders between codes, both neighbours of them, the block's largest below and above a power
+    of two, subnormal blocks, zeros of both signs, infinities and NaN."""
+    x = r.standard_normal((rows, k)).astype(np.float32)
+    b = x.reshape(-1, 32)
+    for i in range(len(b)):
+        kind = i % 9
+        if kind == 1:
+            mids = np.concatenate([(mx.GRID4[1:] + mx.GRID4[:-1]) / 2, mx.GRID4, [7, 7.99]])
+            b[i] = r.choice(mids, 32) * r.choice([-1, 1], 32) * 2.0 ** int(r.integers(-20, 20))
+        elif kind == 2:
+            mids = np.concatenate([(mx.GRID8[1:] + mx.GRID8[:-1]) / 2, [448, 449, 460, 511]]).astype(np.float32)
+            m = r.choice(mids, 32)
+            b[i] = np.where(r.random(32) < 0.5, m, np.nextafter(m, np.float32(r.choice([0, 1e9]))))
+        elif kind == 3:
+            b[i] = np.nextafter(np.float32(2.0 ** int(r.integers(-10, 10))), np.float32(r.choice([0, 1e9]))) * r.choice([1, -1, 0.25], 32)
+        elif kind == 4:
+            b[i] = 0
+            b[i, 3] = -0.0
+        elif kind == 5:
+            b[i] *= np.float32(2.0 ** -120) * np.float32(2.0 ** -int(r.integers(0, 28)))
+        elif kind == 6:
+            b[i] = np.clip(b[i], -1, 1) * np.float32(3.4e38)
+        elif kind == 7 and i % 2:
+            b[i, int(r.integers(32))] = r.choice([np.inf, -np.inf, np.nan])
+    return x
+
+
+@pytest.mark.parametrize("rows,k", [(1, 32), (3, 96), (5, 896), (257, 4896), (1, 18944)])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_weights_round_to_mxfp4(lib, rows, k, t):
+    r = rng(1, rows, k)
+    with np.errstate(over="ignore"):
+        src = half_types(hard_values(r, rows, k), t)
+    codes, scales = guarded(lib, rows * k // 2), guarded(lib, rows * k // 32)
+    lib.quantize_mxfp4(lib.to_device(src), {"f32": 0, "f16": 1, "bf16": 2}[t], codes, scales, rows, k)
+    want_c, want_s = mx.quantize(widened(src, t), True)
+    assert np.array_equal(taken(scales, rows * k // 32, np.uint8, (rows, k // 32)), want_s)
+    assert np.array_equal(taken(codes, rows * k // 2, np.uint8, (rows, k // 2)), mx.pack(want_c))
+
+
+@pytest.mark.parametrize("rows,k", [(1, 32), (3, 96), (5, 896), (257, 4896), (1, 18944)])
+def test_rows_round_to_mxfp8(lib, rows, k):
+    x = hard_values(rng(2, rows, k), rows, k)
+    codes, scales = guarded(lib, rows * k), guarded(lib, rows * k // 32)
+    lib.quantize_mxfp8(lib.to_device(x), codes, scales, rows, k)
+    want_c, want_s = mx.quantize(x, False)
+    assert np.array_equal(taken(scales, rows * k // 32, np.uint8, (rows, k // 32)), want_s)
+    assert np.array_equal(taken(codes, rows * k, np.uint8, (rows, k)), want_c)
+
+
+@pytest.mark.parametrize("four", [True, False])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_values_of_every_code_under_every_scale(lib, four, bf16):
+    """bf16: a scale of 3 and more, below which e4m3's subnormals are rounded. Beyond f32's range: infinity."""
+    scales = np.arange(3, 256, dtype=np.uint8).repeat(16 if not four else 1).reshape(-1, 1)
+    n = len(scales)
+    codes = np.tile(np.arange(256, dtype=np.uint8).reshape(8, 32), (n // 8 + 1, 1))[:n] if not four else np.tile(np.arange(32, dtype=np.uint8) & 15, (n, 1))
+    want = mx.values(codes, scales, four)
+    out = guarded(lib, n * 32 * (2 if bf16 else 4))
+    dc, ds = lib.to_device(mx.pack(codes) if four else codes), lib.to_device(scales)
+    (lib.dequantize_mxfp4 if four else lib.dequantize_mxfp8)(dc, ds, out, lib.T_BF16 if bf16 else lib.T_F32, n, 32)
+    got = taken(out, n * 32 * (2 if bf16 else 4), np.uint16 if bf16 else np.float32, (n, 32))
+    got = widened(got, "bf16") if bf16 else got
+    with np.errstate(over="ignore"):
+        assert np.array_equal(got, want.astype(np.float32), equal_nan=True)
+
+
+@pytest.mark.parametrize("rows,n,S", [(1, 32, 0), (1, 896, 1), (3, 896, 0), (301, 3584, 3), (2, 4896, 64), (70, 96, 2), (1, 18944, 1), (2, 32768, 0)])
+@pytest.mark.parametrize("out", ["apart", "in place", "none"])
+def test_norm_to_mxfp8(lib, rows, n, S, out):
+    r = rng(3, rows, n)
+    x, w = activations(r, rows, n), (1 + 0.1 * r.standard_normal(n)).astype(np.float32)
+    parts = r.standard_normal((S, rows, n)).astype(np.float32)
+    want_x, h = mx.norm(x, parts, w, EPS)
+    want_c, want_s = mx.quantize(h, False)
+    dx = lib.to_device(x)
+    xout = {"apart": lib.empty((rows, n)), "in place": dx, "none": None}[out]
+    codes, scales = guarded(lib, rows * n), guarded(lib, rows * n // 32)
+    lib.rmsnorm_res_mxfp8(dx, lib.to_device(parts) if S else None, S, lib.to_device(w), xout, codes, scales, n, EPS, rows)
+    if xout is not None:
+        assert np.array_equal(xout.numpy().reshape(rows, n), want_x)
+    assert np.array_equal(taken(scales, rows * n // 32, np.uint8, (rows, n // 32)), want_s)
+    assert np.array_equal(taken(codes, rows * n, np.uint8, (rows, n)), want_c)
+
+
+def test_norm_of_rows_that_are_zero_infinite_or_not_a_number(lib):
+    r = rng(4)
+    x = r.standard_normal((5, 896)).astype(np.float32)
+    x[1], x[2, 7], x[3, 890] = 0, np.inf, np.nan
+    w = np.ones(896, np.float32)
+    codes, scales = lib.empty_bytes(5 * 896), lib.empty_bytes(5 * 28)
+    lib.rmsnorm_res_mxfp8(lib.to_device(x), None, 0, lib.to_device(w), None, codes, scales, 896, EPS, 5)
+    with np.errstate(invalid="ignore"):
+        want_c, want_s = mx.quantize(mx.norm(x, [], w, EPS)[1], False)
+    assert np.array_equal(scales.numpy().reshape(5, 28), want_s)
+    assert np.array_equal(codes.numpy().reshape(5, 896), want_c)
+
+
+# Few and many rows, one block of K, K that is no multiple of 128 or 512, features that are no multiple of anything
+SHAPES = [(1, 1, 32), (1, 17, 64), (2, 33, 96), (3, 5, 928), (5, 130, 1152), (7, 4608, 896), (15, 96, 4896), (16, 64, 512), (17, 65, 544),
+          (31, 257, 160), (33, 100, 4864), (64, 896, 896), (65, 129, 288), (77, 896, 4864), (100, 1, 992), (129, 384, 2080), (200, 1000, 416),
+          (257, 515, 896), (301, 600, 1120), (513, 300, 640), (130, 3584, 1184), (1, 3584, 18944), (40, 640, 18944)]
+
+
+def product_bound(a, w, K):
+    return (128 + K / 128 + 64) * 2.0 ** -24 * (np.abs(a) @ np.abs(w).T)
+
+
+def upload_rows(lib, codes, scales, four=False):
+    return lib.to_device(mx.pack(codes) if four else codes), lib.to_device(scales)
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_product(lib, M, N, K):
+    r = rng(5, M, N, K)
+    (ac, asc), (wc, wsc) = rows8(r, M, K), weight(r, N, K)
+    a, w = mx.values(ac, asc, False), mx.values(wc, wsc, True)
+    out = guarded(lib, M * N * 4)
+    before = lib.census()["gemm_mxfp4"]
+    lib.gemm_mxfp4_nt(*upload_rows(lib, ac, asc), *upload_rows(lib, wc, wsc, True), out, M, N, K)
+    assert lib.census()["gemm_mxfp4"] == before + 1
+    got = taken(out, M * N * 4, np.float32, (M, N))
+    assert (np.abs(got - a @ w.T) <= product_bound(a, w, K)).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 17, 64), (7, 896, 4864), (64, 100, 2080), (130, 640, 4896), (257, 515, 896)])
+@pytest.mark.parametrize("room", [1, 3, 16])
+def test_product_as_parts(lib, M, N, K, room):
+    r = rng(6, M, N, K)
+    (ac, asc), (wc, wsc) = rows8(r, M, K), weight(r, N, K)
+    a, w = mx.values(ac, asc, False), mx.values(wc, wsc, True)
+    parts = guarded(lib, room * M * N * 4)
+    parts.nbytes -= 256
+    n = lib.gemm_mxfp4_nt_parts(*upload_rows(lib, ac, asc), *upload_rows(lib, wc, wsc, True), parts, M, N, K)
+    parts.nbytes += 256
+    assert 1 <= n <= room
+    got = taken(parts, room * M * N * 4, np.float32, (room, M, N))
+    assert (got[n:].view(np.uint32) == 0xa5a5a5a5).all(), "more parts than were told"
+    total = got[:n].astype(np.float64).sum(0)
+    assert (np.abs(total - a @ w.T) <= product_bound(a, w, K)).all()
+
+
+def check_gated(got_c, got_s, a, w, K):
+    """Elements next to a border may fall on its other side, and blocks whose largest is next to a power of two may have the other
+    scale: by as much as the product's bound (a gate's slope is below 1.1, so it and the up value each pass on theirs)."""
+    gu = a @ w.T
+    bound = product_bound(a, w, K)
+    ff = gu.shape[1] // 2
+    act = mx.swiglu(gu)
+    # |d act| <= 1.1 |up| d gate + |silu(gate)| d up, and eight roundings of the gate's own arithmetic
+    off = 1.1 * np.abs(gu[:, ff:]) * bound[:, :ff] + np.abs(act / np.where(gu[:, ff:] == 0, 1, gu[:, ff:])) * bound[:, ff:] + np.abs(act) * 2.0 ** -20 + 1e-37
+    v = mx.values(got_c, got_s, False)
+    # a value in [448, 512) times the scale became 448; one rounding of the element: half a step, of the value or of the lowest exponent's
+    step = np.maximum(np.abs(act) * 2.0 ** -4, (2.0 ** (got_s.astype(np.float64) - 127) * 2.0 ** -10).repeat(32, 1))
+    top = (2.0 ** (got_s.astype(np.float64) - 127) * 448).repeat(32, 1)
+    err = np.abs(v - act) - np.where(np.abs(act) > top, np.abs(act) - top, 0)
+    assert (err <= step + off).all()
+    # the scale itself: of the largest magnitude, which is known to within `off`
+    big = np.abs(act).reshape(len(act), -1, 32).max(-1)
+    o = off.reshape(len(act), -1, 32).max(-1)
+    lo, hi = (np.maximum(np.floor(np.log2(np.maximum(b, 2.0 ** -140))) + 119, 0) for b in (big - o, big + o))
+    assert ((lo <= got_s) & (got_s <= hi)).all()
+    # and nearly all are what 64 bits give
+    want_c, want_s = mx.quantize(act.astype(np.float32), False)
+    assert (want_s != got_s).mean() < 0.01 and (want_c != got_c)[(want_s == got_s).repeat(32, 1)].mean() < 0.01
+
+
+@pytest.mark.parametrize("M,ff,K", [(1, 32, 32), (1, 4864, 896), (3, 96, 544), (16, 64, 512), (17, 160, 928), (40, 416, 4896), (77, 1216, 896),
+                                    (130, 352, 1152), (257, 608, 416), (301, 4864, 896), (513, 96, 640)])
+def test_gated_product_to_mxfp8(lib, M, ff, K):
+    r = rng(7, M, ff, K)
+    (ac, asc), (wc, wsc) = rows8(r, M, K), weight(r, 2 * ff, K)
+    wsc = (wsc + 3).astype(np.uint8)          # (gates of order one: both of the sigmoid's sides)
+    codes, scales = guarded(lib, M * ff), guarded(lib, M * ff // 32)
+    lib.gemm_mxfp4_nt_swiglu(*upload_rows(lib, ac, asc), *upload_rows(lib, wc, wsc, True), codes, scales, M, ff, K)
+    check_gated(taken(codes, M * ff, np.uint8, (M, ff)), taken(scales, M * ff // 32, np.uint8, (M, ff // 32)),
+                mx.values(ac, asc, False), mx.values(wc, wsc, True), K)
+
+
+TOKENS = [(1, 32), (3, 64), (17, 96), (16, 512), (896, 896), (1000, 544), (33, 4896), (896, 4864), (4608, 3584), (257, 18944), (20000, 160)]
+
+
+@pytest.mark.parametrize("N,K", TOKENS)
+def test_token_product(lib, N, K):
+    r = rng(8, N, K)
+    x, (wc, wsc) = activations(r, 1, K), weight(r, N, K)
+    w = mx.values(wc, wsc, True)
+    out = guarded(lib, 4 * N)
+    lib.gemv_mxfp4(lib.to_device(x), *upload_rows(lib, wc, wsc, True), out, N, K)
+    got = taken(out, 4 * N, np.float32, (N,))
+    big = np.abs(x[0].astype(np.float64)).reshape(-1, 32).max(-1).repeat(32)
+    bound = product_bound(x.astype(np.float64), w, K)[0] + 2.0 ** -38 * (np.abs(w) @ big)
+    assert (np.abs(got - w @ x[0].astype(np.float64)) <= bound).all()
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e12, 1e30])
+def test_token_product_of_small_and_large_numbers(lib, scale):
+    r = rng(9)
+    x, (wc, wsc) = activations(r, 1, 896) * np.float32(scale), weight(r, 100, 896)
+    w = mx.values(wc, wsc, True)
+    out = lib.empty(100)
+    lib.gemv_mxfp4(lib.to_device(x), *upload_rows(lib, wc, wsc, True), out, 100, 896)
+    big = np.abs(x[0].astype(np.float64)).reshape(-1, 32).max(-1).repeat(32)
+    bound = product_bound(x.astype(np.float64), w, 896)[0] + 2.0 ** -38 * (np.abs(w) @ big)
+    assert (np.abs(out.numpy() - w @ x[0].astype(np.float64)) <= bound).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 70, 416), (200, 300, 928)])
+def test_not_a_number_stays_with_its_row(lib, M, N, K):
+    """A block with scale 255, or an element that is NaN, makes its own row of the result NaN and no other; blocks at the ends of the
+    rows are what the tiles' edges read."""
+    r = rng(10, M, N)
+    (ac, asc), (wc, wsc) = rows8(r, M, K), weight(r, N, K)
+    clean = mx.values(ac, asc, False) @ mx.values(wc, wsc, True).T
+    asc[M - 1, -1], wsc[2, 0], ac[1, K - 1] = 255, 255, 0x7f
+    wsc[N - 1, -1] = 255
+    out = lib.empty((M, N))
+    lib.gemm_mxfp4_nt(*upload_rows(lib, ac, asc), *upload_rows(lib, wc, wsc, True), out, M, N, K)
+    got = out.numpy()
+    nan = np.zeros((M, N), bool)
+    nan[[1, M - 1]] = True
+    nan[:, [2, N - 1]] = True
+    assert np.array_equal(np.isnan(got), nan)
+    assert np.allclose(got[~nan], clean[~nan], rtol=1e-4, atol=1e-4 * np.abs(clean).max())
+    y = lib.empty(N)
+    lib.gemv_mxfp4(lib.to_device(activations(r, 1, K)), *upload_rows(lib, wc, wsc, True), y, N, K)
+    assert np.array_equal(np.isnan(y.numpy()), nan[0])
+
+
+@pytest.mark.parametrize("M", [1, 9, 77])
+def test_layer_of_a_prompt(lib, M):
+    """The calls of a feed-forward layer one after the other: norm, gated product, down projection in parts, norm of the next
+    layer; each held to 64 bits on what the call before it wrote."""
+    r = rng(11, M)
+    E, F = 896, 1216
+    x, w1, w2 = activations(r, M, E), (1 + 0.1 * r.standard_normal(E)).astype(np.float32), (1 + 0.1 * r.standard_normal(E)).astype(np.float32)
+    (gc, gs), (dc, ds) = weight(r, 2 * F, E), weight(r, E, F)
+    hc, hs, fc, fs = (lib.empty_bytes(n) for n in (M * E, M * E // 32, M * F, M * F // 32))
+    dx, parts = lib.to_device(x), lib.empty((8, M, E))
+    lib.rmsnorm_res_mxfp8(dx, None, 0, lib.to_device(w1), None, hc, hs, E, EPS, M)
+    lib.gemm_mxfp4_nt_swiglu(hc, hs, *upload_rows(lib, gc, gs, True), fc, fs, M, F, E)
+    n = lib.gemm_mxfp4_nt_parts(fc, fs, *upload_rows(lib, dc, ds, True), parts, M, E, F)
+    first = hc.numpy().reshape(M, E), hs.numpy().reshape(M, -1)
+    lib.rmsnorm_res_mxfp8(dx, parts, n, lib.to_device(w2), dx, hc, hs, E, EPS, M)
+    want = mx.quantize(mx.norm(x, [], w1, EPS)[1], False)
+    assert np.array_equal(first[0], want[0]) and np.array_equal(first[1], want[1])
+    f = fc.numpy().reshape(M, F), fs.numpy().reshape(M, -1)
+    check_gated(*f, mx.values(*first, False), mx.values(gc, gs, True), E)
+    p = parts.numpy()[:n]
+    a, w = mx.values(*f, False), mx.values(dc, ds, True)
+    assert (np.abs(p.astype(np.float64).sum(0) - a @ w.T) <= product_bound(a, w, F)).all()
+    want_x, h = mx.norm(x, p, w2, EPS)
+    want = mx.quantize(h, False)
+    assert np.array_equal(dx.numpy().reshape(M, E), want_x)
+    assert np.array_equal(hc.numpy().reshape(M, E), want[0]) and np.array_equal(hs.numpy().reshape(M, -1), want[1])
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 896, 4864), (7, 896, 4864), (33, 416, 2080), (130, 896, 4864)])
+def test_recorded_product(fresh_lib, recorded, M, N, K):
+    """Recorded ahead of any eager call, replayed with other work between: what the eager call gives, or its parts in another
+    order."""
+    lib, r = fresh_lib, rng(12, M)
+    (ac, asc), (wc, wsc) = rows8(r, M, K), weight(r, N, K)
+    a, w = mx.values(ac, asc, False), mx.values(wc, wsc, True)
+    da, dw, out = upload_rows(lib, ac, asc), upload_rows(lib, wc, wsc, True), lib.empty((M, N))
+    for got in recorded(lambda: lib.gemm_mxfp4_nt(*da, *dw, out, M, N, K), out):
+        assert (np.abs(got.reshape(M, N) - a @ w.T) <= product_bound(a, w, K)).all()
+
+
+def test_recorded_layer(fresh_lib, recorded):
+    lib, r = fresh_lib, rng(13)
+    M, E, F = 33, 896, 608
+    x, nw = lib.to_device(activations(r, M, E)), lib.to_device(np.ones(E, np.float32))
+    g, d = upload_rows(lib, *weight(r, 2 * F, E), True), upload_rows(lib, *weight(r, E, F), True)
+    hc, hs, fc, fs = (lib.empty_bytes(n) for n in (M * E, M * E // 32, M * F, M * F // 32))
+    y, tok, row = lib.empty((M, E)), lib.empty(E), lib.to_device(activations(r, 1, F))
+    both = lib.empty(M * E + E)
+
+    def layer():
+        lib.rmsnorm_res_mxfp8(x, None, 0, nw, None, hc, hs, E, EPS, M)
+        lib.gemm_mxfp4_nt_swiglu(hc, hs, *g, fc, fs, M, F, E)
+        lib.gemm_mxfp4_nt(fc, fs, *d, y, M, E, F)
+        lib.gemv_mxfp4(row, *d, tok, E, F)
+        lib._chk(lib.c.tlhip_memcpy_d2d_async(both.ptr, y.ptr, y.nbytes))
+        lib._chk(lib.c.tlhip_memcpy_d2d_async(both.ptr + y.nbytes, tok.ptr, tok.nbytes))
+
+    replays = recorded(layer, both)
+    layer()
+    lib.sync()
+    eager = both.numpy()
+    scale = np.abs(eager).max()
+    for got in replays:
+        assert np.abs(got - eager).max() <= 1e-5 * scale
+    assert np.array_equal(replays[0], replays[1]) and np.array_equal(replays[0], replays[2])
+
+
+def test_products_are_deterministic(lib):
+    r = rng(14)
+    for M, N, K in [(1, 4608, 3584), (7, 896, 4864), (129, 896, 4864)]:
+        (ac, asc), (wc, wsc) = rows8(r, M, K), weight(r, N, K)
+        da, dw, out = upload_rows(lib, ac, asc), upload_rows(lib, wc, wsc, True), lib.empty((M, N))
+        got = []
+        for _ in range(3):
+            lib.gemm_mxfp4_nt(*da, *dw, out, M, N, K)
+            got.append(out.numpy())
+        assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+
+
+def test_refusals(lib):
+    b, odd = lib.empty_bytes(1 << 16), C.c_void_p(0)
+    p, n = b.ptr, C.c_int(0)
+    odd = p + 4
+    EINVAL, EUNSUPPORTED = -2, -3
+    c = lib.c
+    cases = [
+        (c.tlhip_quantize_mxfp4, (None, 0, p, p, 1, 32), EINVAL), (c.tlhip_quantize_mxfp4, (p, 3, p, p, 1, 32), EUNSUPPORTED),
+        (c.tlhip_quantize_mxfp4, (p, 0, p, p, 0, 32), EINVAL), (c.tlhip_quantize_mxfp4, (p, 0, p, p, 1, 33), EINVAL),
+        (c.tlhip_quantize_mxfp4, (p, 0, p, p, 1, 0), EINVAL), (c.tlhip_quantize_mxfp4, (odd, 0, p, p, 1, 32), EINVAL),
+        (c.tlhip_quantize_mxfp4, (p, 0, odd, p, 1, 32), EINVAL), (c.tlhip_quantize_mxfp4, (p, 0, p, p, 1 << 62, 1 << 20), EUNSUPPORTED),
+        (c.tlhip_quantize_mxfp8, (p, None, p, 1, 32), EINVAL), (c.tlhip_quantize_mxfp8, (p, p, p, 1, 16), EINVAL),
+        (c.tlhip_quantize_mxfp8, (p, p, p, -1, 32), EINVAL), (c.tlhip_quantize_mxfp8, (p, odd, p, 1, 32), EINVAL),
+        (c.tlhip_dequantize_mxfp4, (p, p, p, 1, 1, 32), EUNSUPPORTED), (c.tlhip_dequantize_mxfp4, (p, None, p, 0, 1, 32), EINVAL),
+        (c.tlhip_dequantize_mxfp8, (p, p, odd, 0, 1, 32), EINVAL), (c.tlhip_dequantize_mxfp8, (p, p, p, 0, 1, 40), EINVAL),
+        (c.tlhip_rmsnorm_res_mxfp8, (p, None, 1, p, None, p, p, 32, 1e-6, 1), EINVAL),
+        (c.tlhip_rmsnorm_res_mxfp8, (p, p, 1, p, p, p, p, 32, 1e-6, 1), EINVAL),
+        (c.tlhip_rmsnorm_res_mxfp8, (p, None, 0, p, None, p, p, 40, 1e-6, 1), EINVAL),
+        (c.tlhip_rmsnorm_res_mxfp8, (p, None, 0, p, None, p, p, 32800, 1e-6, 1), EUNSUPPORTED),
+        (c.tlhip_rmsnorm_res_mxfp8, (p, p, 65, p, None, p, p, 32, 1e-6, 1), EUNSUPPORTED),
+        (c.tlhip_rmsnorm_res_mxfp8, (p, p, -1, p, None, p, p, 32, 1e-6, 1), EUNSUPPORTED),
+        (c.tlhip_rmsnorm_res_mxfp8, (p, None, 0, p, odd, p, p, 32, 1e-6, 1), EINVAL),
+        (c.tlhip_rmsnorm_res_mxfp8, (p, None, 0, p, None, p, p, 32, 1e-6, 0), EINVAL),
+        (c.tlhip_gemv_mxfp4, (p, p, p, None, 1, 32), EINVAL), (c.tlhip_gemv_mxfp4, (p, p, p, p, 1, 48), EINVAL),
+        (c.tlhip_gemv_mxfp4, (p, odd, p, p, 1, 32), EINVAL), (c.tlhip_gemv_mxfp4, (p, p, p, p, 0, 32), EINVAL),
+        (c.tlhip_gemv_mxfp4, (p, p, p, p, 1 << 40, 32), EUNSUPPORTED),
+        (c.tlhip_gemm_mxfp4_nt, (p, None, p, p, p, 1, 1, 32), EINVAL), (c.tlhip_gemm_mxfp4_nt, (p, p, p, p, p, 0, 1, 32), EINVAL),
+        (c.tlhip_gemm_mxfp4_nt, (p, p, p, p, p, 1, 1, 31), EINVAL), (c.tlhip_gemm_mxfp4_nt, (odd, p, p, p, p, 1, 1, 32), EINVAL),
+        (c.tlhip_gemm_mxfp4_nt, (p, p, p, p, p, 1 << 30, 1, 32), EUNSUPPORTED),
+        (c.tlhip_gemm_mxfp4_nt_parts, (p, p, p, p, p, 255, 2, 32, 32, C.byref(n)), EINVAL),
+        (c.tlhip_gemm_mxfp4_nt_parts, (p, p, p, p, p, 256, 2, 32, 32, None), EINVAL),
+        (c.tlhip_gemm_mxfp4_nt_swiglu, (p, p, p, p, p, p, 1, 33, 32), EINVAL),
+        (c.tlhip_gemm_mxfp4_nt_swiglu, (p, p, p, p, p, None, 1, 32, 32), EINVAL),
+        (c.tlhip_gemm_mxfp4_nt_swiglu, (p, p, p, p, odd, p, 1, 32, 32), EINVAL),
+    ]
+    before = lib.census()
+    for fn, args, want in cases:
+        assert fn(*args) == want, (fn.__name__, args)
+        assert lib.last_error().startswith(fn.__name__)
+    assert lib.census() == before
