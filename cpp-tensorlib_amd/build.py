@@ -16,7 +16,7 @@ OBJDIR = os.path.join(HERE, "build")
 LIB = os.path.join(LIBDIR, "libtensorlib_hip.so")
 SOURCES = ["runtime.hip", "gemv.hip", "elementwise.hip", "modelops.hip", "attn.hip", "attn_prefill_mfma.hip", "attn_prefill_f16.hip", "prefill.hip", "gemm_rows.hip", "gemm_q4.hip", "gemm_f16t.hip", "convert.hip", "sgemm.hip", "sgemm_split.hip",
            "attn_window.hip", "linear_attn.hip", "hybrid_step.hip", "seqops.hip",
-           "ssm.hip", "latent_attn.hip", "mx_quant.hip", "gemm_mx.hip"]
+           "ssm.hip", "latent_attn.hip", "mx_quant.hip", "gemm_mx.hip", "gemv_mx.hip"]
 # -packed-fp32-ops off: some forms of v_pk_*_f32 have given wrong results now and then; hipcc must not form them.
 # Preloaded kernel arguments: the command processor puts a kernel's first 14 dwords of arguments into scalar registers while the
 # launch before it still runs, where a load of them is the first thing that a block waits for (a chain of kernels of 4 us each, with

@@ -153,6 +153,8 @@ SIGNATURES = {
     "tlhip_dequantize_mxfp8": (cint, [P, P, P, cint, i64, i64]),
     "tlhip_rmsnorm_res_mxfp8": (cint, [P, P, i64, P, P, P, P, i64, f32, i64]),
     "tlhip_gemv_mxfp4": (cint, [P, P, P, P, i64, i64]),
+    "tlhip_gemv_mxfp4_rmsnorm": (cint, [P, P, P, P, P, P, P, i64, i64, f32]),
+    "tlhip_gemv_mxfp4_rmsnorm_gateup": (cint, [P, P, P, P, P, P, P, i64, i64, f32]),
     "tlhip_gemm_mxfp4_nt": (cint, [P, P, P, P, P, i64, i64, i64]),
     "tlhip_gemm_mxfp4_nt_parts": (cint, [P, P, P, P, P, i64, i64, i64, i64, P]),
     "tlhip_gemm_mxfp4_nt_swiglu": (cint, [P, P, P, P, P, P, i64, i64, i64]),
@@ -590,6 +592,14 @@ class TlHip:
 
     def gemv_mxfp4(self, a, codes, scales, y, N, K):
         self._chk(self.c.tlhip_gemv_mxfp4(a.ptr, codes.ptr, scales.ptr, y.ptr, N, K))
+
+    def gemv_mxfp4_rmsnorm(self, x, delta, norm_w, xout, codes, scales, y, N, K, eps):
+        self._chk(self.c.tlhip_gemv_mxfp4_rmsnorm(x.ptr, delta.ptr if delta is not None else None, norm_w.ptr,
+                                                  xout.ptr if xout is not None else None, codes.ptr, scales.ptr, y.ptr, N, K, eps))
+
+    def gemv_mxfp4_rmsnorm_gateup(self, x, delta, norm_w, xout, codes, scales, act, N2, K, eps):
+        self._chk(self.c.tlhip_gemv_mxfp4_rmsnorm_gateup(x.ptr, delta.ptr if delta is not None else None, norm_w.ptr,
+                                                         xout.ptr if xout is not None else None, codes.ptr, scales.ptr, act.ptr, N2, K, eps))
 
     def gemm_mxfp4_nt(self, acodes, ascales, codes, scales, out, M, N, K):
         self._chk(self.c.tlhip_gemm_mxfp4_nt(acodes.ptr, ascales.ptr, codes.ptr, scales.ptr, out.ptr, M, N, K))

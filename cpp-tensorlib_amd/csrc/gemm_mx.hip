@@ -1,195 +1,280 @@
-// Products over MXFP4 weights (mx_formats.hpp): of one f32 row, and of MXFP8 rows, on the scaled matrix instructions.
-//
-// C[m][n] = sum over blocks b of 2^(sa + sw - 254) sum over 32 of a w: v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 rows of
-// 128 e2m1 elements by 16 rows of 128 e4m3 ones, each block of 32 with its own scale byte, into f32 sums. Lane l holds row l % 16 of both
-// operands; with g = l / 16 its 16 bytes of e2m1 are k = 32 g .. 32 g + 31, its 32 bytes of e4m3 k = 16 g .. + 15 and 64 + 16 g
-// .. + 15, and its scale bytes are those of block g. The weight is the first operand: lane l's four results are features 4 g .. 4 g + 3 of token
-// l % 16, one 16-byte store.
-//
-// The instruction adds the products of eight neighbouring k to the precision of the largest of them: whatever of a product lies
-// more than 13 binades below the sum of that one's exponents is cut off (measured: 2688 + 0.125 keeps the 0.125, 2688 + 0.0625
-// does not; a random product over 18944 is 1.4e-5 off, f32 sums 3e-8). e4m3 spans 18 binades, so activations go in twice, the elements of
-// at least 2 (bit 6 of the byte: exponent field 8 to 15) and the others apart. Of the first a product's last bit is 2^-2 x 2^-1 at
-// least, the largest exponents add up to 8 + 2; of the others 2^-9 x 2^-1 and 0 + 2: nothing is cut off in either, and sums
-// of eight and more are f32. Half the instruction's rate is what that costs.
-#include "mx_formats.hpp"
-#include "gemv_shared.hpp"
+// Products of MXFP8 rows over MXFP4 weights, in tiles: prompt chunks, plain, as the parts of a split K, and with the gated activation whose
+// result is MXFP8 again (mx_mfma.hpp has the arithmetic).
+#include "mx_mfma.hpp"
 
 #include <algorithm>
 
 namespace tlhip {
 
-__device__ __forceinline__ v4f mx_mma(const v8i w, const v8i a, const v4f c, int sw, int sa) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 4, 0, 0, sw, 0, sa);
-}
-
-// Keeps the instructions that formed c ahead of what follows. They read the registers of all 64 lanes, but the compiler holds them
-// to be free to move: where only some lanes need a result it has put one under their branch, operands prepared there for
-// those lanes only.
-__device__ __forceinline__ void mx_done(v4f& c) { asm volatile("" : "+v"(c)); }
-
-// The elements of at least 2 of a register of e4m3, and the others (zeros elsewhere, signs in both)
-__device__ __forceinline__ void split_e4m3(const v8i a, v8i& large, v8i& small) {
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const uint32_t w = (uint32_t)a[i], t = w & 0x40404040u;
-    const uint32_t keep = (t << 1) + (0x80808080u - (t >> 6));        // bytes 0xff where bit 6 is set, else 0x80
-    large[i] = (int)(w & keep);
-    small[i] = (int)(w & (~keep | 0x80808080u));
+// ---- tiles: many rows ---------------------------------------------------------------------------------------------
+// WF x WT wavefronts, each NF x NT tiles of 16 features by 16 tokens. A step is 128 k: the rows' bytes and scales go from memory into LDS
+// by copies, a step ahead; 16-byte chunks of a row are swizzled on the memory side of the copy, so that the lanes an LDS read
+// serves together find different banks. A row's four scale bytes of a step are one word, which a lane shifts down to its own block's.
+// WORDS: that word is a whole one in memory, too (K % 128 == 0, so that no step ends past a row); elsewhere it is read
+// from wherever it lies.
+typedef uint32_t any4 __attribute__((aligned(1)));
+__device__ __forceinline__ uint32_t four_scales(const uint8_t* row, int b, int nb) {      // bytes b .. b + 3 of nb, 0 past them (b < nb)
+  if (nb < 4) {
+    uint32_t v = row[0];
+    if (nb > 1) v |= (uint32_t)row[1] << 8;
+    if (nb > 2) v |= (uint32_t)row[2] << 16;
+    return v;
   }
+  const int at = min(b, nb - 4);
+  return *reinterpret_cast<const any4*>(row + at) >> (8 * (b - at));
 }
-__device__ __forceinline__ v4f mx_mma_both(const v8i w, const v8i a, v4f c, int sw, int sa) {
-  v8i large, small;
-  split_e4m3(a, large, small);
-  c = mx_mma(w, small, c, sw, sa);
-  return mx_mma(w, large, c, sw, sa);
-}
+struct MxTiles {
+  int tokens, count;       // tiles of tokens, all tiles
+  int parts, steps;        // K split: parts of so many steps of 128
+};
 
-// One wavefront: 16 features (GU: 32 gate and the 32 up ones) by 16 tokens, operands straight from memory.
-// What lies past the end of a row is the row's last block again under the scale 2^-127 on both sides: 2^-254 times at most 32 x 448 x 6,
-// which is 0 in f32.
-struct MxFrag { v8i v; int s; };
-__device__ __forceinline__ MxFrag mx_weight(const uint8_t* W, const uint8_t* scales, int64_t row, int nb, int b) {
-  const int at = min(b, nb - 1);
-  const uint4 c = *reinterpret_cast<const uint4*>(W + (row * nb + at) * 16);
-  return MxFrag{v8i{(int)c.x, (int)c.y, (int)c.z, (int)c.w, 0, 0, 0, 0}, b < nb ? (int)scales[row * nb + at] : 0};
-}
-__device__ __forceinline__ MxFrag mx_act(const uint8_t* A, const uint8_t* scales, int64_t row, int nb, int b0, int g) {
-  const int64_t K = (int64_t)nb * 32;
-  const int c0 = min(2 * b0 + g, 2 * nb - 1), c1 = min(2 * b0 + 4 + g, 2 * nb - 1);        // 16-byte chunks of the row
-  const uint4 lo = *reinterpret_cast<const uint4*>(A + row * K + 16 * c0), hi = *reinterpret_cast<const uint4*>(A + row * K + 16 * c1);
-  return MxFrag{v8i{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w},
-                b0 + g < nb ? (int)scales[row * nb + b0 + g] : 0};
-}
+template <int WF, int WT, int NF, int NT, int WPE, bool GATED, bool WORDS>
+__global__ __launch_bounds__(64 * WF * WT, WPE) void mx_tile_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ sa,
+                                                                    const uint8_t* __restrict__ W, const uint8_t* __restrict__ sw, int M, int N, int nb,
+                                                                    MxTiles P, float* __restrict__ C, uint8_t* __restrict__ codes,
+                                                                    uint8_t* __restrict__ scales) {
+  constexpr int kWaves = WF * WT, kThreads = 64 * kWaves, TF = 16 * NF * WF, TT = 16 * NT * WT, kRows = TF + TT;
+  constexpr int kWBytes = TF * 64, kElems = kWBytes + TT * 128, kStage = kElems + kRows * 4;
+  constexpr int kCopies = kElems / 1024 / kWaves, kRowsEach = (kRows + kThreads - 1) / kThreads;
+  static_assert(kElems % (1024 * kWaves) == 0 && kWBytes % (1024 * kWaves) == 0 && kRows % 64 == 0, "whole copies");
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wf = wave / WT, wt = wave % WT;
+  const BlockPlace at = block_place(P.count, P.parts);
+  const int tf = at.tile / P.tokens, tt = at.tile - tf * P.tokens;
+  const int all = (nb + 3) / 4, first = at.part * P.steps, steps = min(P.steps, all - first);
+  // row of the weight for row i of the tile: with a gate, a wavefront's tiles are gate rows, then the up rows of the same features
+  constexpr int kFeatures = GATED ? TF / 2 : TF;
+  const auto weight_row = [&](int i) -> int64_t {
+    if constexpr (!GATED) return min(tf * TF + i, N - 1);
+    const int w = i / (16 * NF), f = i % (16 * NF);
+    return min(tf * kFeatures + w * (8 * NF) + f % (8 * NF), N - 1) + (f < 8 * NF ? (int64_t)0 : (int64_t)N);
+  };
+  const auto token_row = [&](int i) -> int64_t { return min(tt * TT + i, M - 1); };
 
-__global__ __launch_bounds__(64) void mx_gemm_simple_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ sa,
-                                                            const uint8_t* __restrict__ W, const uint8_t* __restrict__ sw,
-                                                            float* __restrict__ C, int M, int N, int nb) {
-  const int lane = threadIdx.x, r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, m = blockIdx.y * 16 + r;
-  const int64_t wr = min(n0 + r, N - 1), ar = min(m, M - 1);
-  v4f c = {0.f, 0.f, 0.f, 0.f};
-  for (int b = 0; b < nb; b += 4) {
-    const MxFrag w = mx_weight(W, sw, wr, nb, b + g), a = mx_act(A, sa, ar, nb, b, g);
-    c = mx_mma_both(w.v, a.v, c, w.s, a.s);
+  // Rows of a wavefront's copies, 16 of the weight or 8 of the activations: the first one's address (uniform) and 32-bit offsets
+  const uint8_t* src[kCopies];
+  uint32_t off[kCopies], chunk[kCopies];
+#pragma unroll
+  for (int j = 0; j < kCopies; j++) {
+    const bool w = j * kWaves * 1024 < kWBytes;
+    const int q = j * kWaves + wave - (w ? 0 : kWBytes / 1024), row0 = q * (w ? 16 : 8), row = row0 + (lane >> (w ? 2 : 3));
+    const int64_t base = w ? weight_row(row0) : token_row(row0), mine = w ? weight_row(row) : token_row(row);
+    src[j] = w ? W + base * nb * 16 : A + base * nb * 32;
+    chunk[j] = (w ? (lane & 3) ^ (-(row >> 2) & 3) : (lane & 7) ^ (row >> 1 & 7)) * 16;
+    off[j] = (uint32_t)(mine - base) * (uint32_t)nb * (w ? 16u : 32u);
   }
-  mx_done(c);
-  if (m >= M) return;
+  const uint8_t* srow[kRowsEach];
+  uint32_t sc[kRowsEach];
 #pragma unroll
-  for (int i = 0; i < 4; i++)
-    if (n0 + 4 * g + i < N) C[(int64_t)m * N + n0 + 4 * g + i] = c[i];
-}
+  for (int j = 0; j < kRowsEach; j++) {
+    const int i = min(j * kThreads + tid, kRows - 1);
+    srow[j] = i < TF ? sw + weight_row(i) * nb : sa + token_row(i - TF) * nb;
+  }
+  const auto copy = [&](int step, int stage) {
+    char* s = lds + stage * kStage;
+    if constexpr (!WORDS) {
+#pragma unroll
+      for (int j = 0; j < kRowsEach; j++) sc[j] = four_scales(srow[j], (first + step) * 4, nb);
+    }
+#pragma unroll
+    for (int j = 0; j < kCopies; j++) {
+      const bool w = j * kWaves * 1024 < kWBytes;
+      uint32_t k = (uint32_t)(first + step) * (w ? 64u : 128u) + chunk[j];
+      if constexpr (!WORDS) k = min(k, (uint32_t)(w ? nb - 1 : 2 * nb - 1) * 16u);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[j] + (off[j] + k)),
+                                       (__attribute__((address_space(3))) void*)(s + (j * kWaves + wave) * 1024), 16, 0, 0);
+    }
+    if constexpr (WORDS) {
+#pragma unroll
+      for (int j = 0; j < kRowsEach; j++)
+        if (j * kThreads + wave * 64 < kRows)
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(srow[j] + (first + step) * 4),
+                                           (__attribute__((address_space(3))) void*)(s + kElems + (j * kThreads + wave * 64) * 4), 4, 0, 0);
+    }
+  };
+  const auto keep_scales = [&](int stage) {      // of the step copied last
+    if constexpr (!WORDS) {
+#pragma unroll
+      for (int j = 0; j < kRowsEach; j++)
+        if (j * kThreads + tid < kRows) *reinterpret_cast<uint32_t*>(lds + stage * kStage + kElems + (j * kThreads + tid) * 4) = sc[j];
+    }
+  };
 
-// 32 features: two tiles of 16; token l % 16's block of 32 activations lies in the four lanes with that l % 16
-__global__ __launch_bounds__(64) void mx_gated_simple_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ sa,
-                                                             const uint8_t* __restrict__ W, const uint8_t* __restrict__ sw,
-                                                             uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int M, int ff, int nb) {
-  const int lane = threadIdx.x, r = lane & 15, g = lane >> 4;
-  const int f0 = blockIdx.x * 32, m = blockIdx.y * 16 + r;
-  const int64_t ar = min(m, M - 1);
-  v4f c[4];
+  v4f c[NF][NT];
 #pragma unroll
-  for (int t = 0; t < 4; t++) c[t] = v4f{0.f, 0.f, 0.f, 0.f};
-  for (int b = 0; b < nb; b += 4) {
-    const MxFrag a = mx_act(A, sa, ar, nb, b, g);
+  for (int f = 0; f < NF; f++)
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-      const MxFrag w = mx_weight(W, sw, f0 + 16 * (t & 1) + r + (t >> 1) * (int64_t)ff, nb, b + g);
-      c[t] = mx_mma_both(w.v, a.v, c[t], w.s, a.s);
+    for (int t = 0; t < NT; t++) c[f][t] = v4f{0.f, 0.f, 0.f, 0.f};
+  // where my operands lie in a stage
+  const int wrow = (wf * 16 * NF + r) * 64 + ((g ^ (-(r >> 2) & 3)) << 4);              // (+ 1024 a tile)
+  const int arow = kWBytes + (wt * 16 * NT + r) * 128, ax = r >> 1 & 7;                 // (+ 2048 a tile)
+  const int a0 = arow + ((g ^ ax) << 4), a1 = arow + (((4 + g) ^ ax) << 4);
+  const int ws = kElems + (wf * 16 * NF + r) * 4, as = kElems + (TF + wt * 16 * NT + r) * 4;   // (+ 64 a tile)
+
+  copy(0, 0);
+  keep_scales(0);
+  for (int i = 0; i < steps; i++) {
+    // what was copied a step ago has landed, my reads are done, and so are everybody's
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (i + 1 < steps) copy(i + 1, (i + 1) & 1);
+    // LDS is read as vectors of words, never as uint4, which the compiler takes for something that a copy in flight may write
+    const char* s = lds + (i & 1) * kStage;
+    frag16 w[NF];
+    int swv[NF];
+#pragma unroll
+    for (int f = 0; f < NF; f++) {
+      w[f] = *reinterpret_cast<const frag16*>(s + wrow + f * 1024);
+      swv[f] = (int)(*reinterpret_cast<const uint32_t*>(s + ws + f * 64) >> (8 * g));
+    }
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const frag16 lo = *reinterpret_cast<const frag16*>(s + a0 + t * 2048), hi = *reinterpret_cast<const frag16*>(s + a1 + t * 2048);
+      const int sav = (int)(*reinterpret_cast<const uint32_t*>(s + as + t * 64) >> (8 * g));
+      v8i large, small;
+      split_e4m3(row_operand(lo, hi), large, small);
+#pragma unroll
+      for (int f = 0; f < NF; f++)
+        c[f][t] = mx_mma(weight_operand(w[f]), small, c[f][t], swv[f], sav);
+#pragma unroll
+      for (int f = 0; f < NF; f++)
+        c[f][t] = mx_mma(weight_operand(w[f]), large, c[f][t], swv[f], sav);
+    }
+    if (i + 1 < steps) keep_scales((i + 1) & 1);
+  }
+#pragma unroll
+  for (int f = 0; f < NF; f++)
+#pragma unroll
+    for (int t = 0; t < NT; t++) mx_done(c[f][t]);
+
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const int m = tt * TT + (wt * NT + t) * 16 + r;
+    if constexpr (!GATED) {
+      float* out = C + ((int64_t)at.part * M + m) * N;
+#pragma unroll
+      for (int f = 0; f < NF; f++)
+        if (m < M) store_features(out, tf * TF + (wf * NF + f) * 16 + 4 * g, N, c[f][t]);
+    } else {
+#pragma unroll
+      for (int p = 0; p < NF / 4; p++) {          // blocks of 32 features: two tiles
+        const int n = tf * kFeatures + wf * (8 * NF) + 32 * p;
+        store_gated(c[2 * p][t], c[2 * p + 1][t], c[NF / 2 + 2 * p][t], c[NF / 2 + 2 * p + 1][t], g, m < M && n < N,
+                    codes + (int64_t)min(m, M - 1) * N + n, scales + (int64_t)min(m, M - 1) * (N / kMxBlock) + n / kMxBlock);
+      }
     }
   }
-#pragma unroll
-  for (int t = 0; t < 4; t++) mx_done(c[t]);
-  float v[8];
-  uint32_t big = 0;
-#pragma unroll
-  for (int t = 0; t < 8; t++) {
-    v[t] = gated(c[t >> 2][t & 3], c[2 + (t >> 2)][t & 3]);
-    big = max(big, magnitude(v[t]));
-  }
-  big = max(big, (uint32_t)__shfl_xor((int)big, 16, kWave));
-  big = max(big, (uint32_t)__shfl_xor((int)big, 32, kWave));
-  const uint32_t s = mx_scale_of(big, kMx8Exp);
-  const float up = mx_up(min(s, 252u));
-#pragma unroll
-  for (int t = 0; t < 8; t++) v[t] = s == 255u ? 0.f : v[t] * up;
-  if (m >= M) return;
-#pragma unroll
-  for (int t = 0; t < 2; t++)
-    *reinterpret_cast<uint32_t*>(codes + (int64_t)m * ff + f0 + 16 * t + 4 * g) = to_e4m3x4(v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]);
-  if (g == 0) scales[(int64_t)m * (ff / kMxBlock) + blockIdx.x] = (uint8_t)s;
 }
 
-// One wavefront a row of the weight
-__global__ __launch_bounds__(256) void mx_gemv_simple_kernel(const float* __restrict__ a, const uint8_t* __restrict__ W,
-                                                             const uint8_t* __restrict__ sw, float* __restrict__ y, int N, int nb) {
-  const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (n >= N) return;
-  float sum = 0.f;
-  for (int b = lane; b < nb; b += 64) {
-    const uint4 c = *reinterpret_cast<const uint4*>(W + (n * nb + b) * 16);
-    const uint32_t d[4] = {c.x, c.y, c.z, c.w};
-    float p = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float* x = a + 32 * b + 8 * i;
-      const v2f w0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d[i], 1.0f, 0), w1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d[i], 1.0f, 1);
-      const v2f w2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d[i], 1.0f, 2), w3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d[i], 1.0f, 3);
-      p = fmaf(w0[0], x[0], fmaf(w0[1], x[1], fmaf(w1[0], x[2], fmaf(w1[1], x[3], p))));
-      p = fmaf(w2[0], x[4], fmaf(w2[1], x[5], fmaf(w3[0], x[6], fmaf(w3[1], x[7], p))));
+template <int WF, int WT, int NF, int NT, int WPE, bool GATED>
+static hipError_t launch_tiles(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N, int64_t K, int parts,
+                               float* C, uint8_t* codes, uint8_t* scales) {
+  constexpr int TF = 16 * NF * WF / (GATED ? 2 : 1), TT = 16 * NT * WT;
+  constexpr int lds = 2 * (16 * NF * WF * 68 + TT * 132);
+  static_assert(lds <= 160 * 1024, "LDS");
+  MxTiles P;
+  P.tokens = (int)((M + TT - 1) / TT);
+  P.count = (int)((N + TF - 1) / TF) * P.tokens;
+  const int all = (int)((K + 127) / 128);
+  P.steps = (all + parts - 1) / parts;
+  P.parts = (all + P.steps - 1) / P.steps;
+  const int nb = (int)(K / kMxBlock);
+  const bool words = nb % 4 == 0 && ((reinterpret_cast<uintptr_t>(sa) | reinterpret_cast<uintptr_t>(sw)) & 3) == 0;
+  const auto kernel = words ? mx_tile_kernel<WF, WT, NF, NT, WPE, GATED, true> : mx_tile_kernel<WF, WT, NF, NT, WPE, GATED, false>;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (e != hipSuccess) return e;
+  kernel<<<dim3((unsigned)P.count, (unsigned)P.parts), dim3(64 * WF * WT), lds, ctx().stream>>>(A, sa, W, sw, (int)M, (int)N, nb, P, C, codes,
+                                                                                                scales);
+  return hipGetLastError();
+}
+
+// ---- which tiles --------------------------------------------------------------------------------------------------------
+// Features x tokens of a tile and its blocks on a CU: 128 x 64 (four), 128 x 128 (three), 256 x 128 (two). A step takes `one` us plus
+// `more` for each block on a CU, as measured on products of 30 to 2048 rows by 896 x 4864 to 37888 x 3584; the launch that adds
+// parts up 2.2 us and their traffic at 5 TB/s.
+struct MxPlan { int variant = 0, parts = 1; double us = 1e30; };
+static const struct { int features, tokens; double one, more; } kVariant[3] = {{128, 64, 0.35, 0.38}, {128, 128, 0.4, 0.72}, {256, 128, 0.9, 1.55}};
+
+static MxPlan plan_tiles(int64_t M, int64_t N, int64_t K, int64_t max_parts, bool gated, bool own_sum) {
+  const int64_t cus = cu_count(), steps = (K + 127) / 128;
+  MxPlan best;
+  for (int v = 0; v < 3; v++) {
+    const int64_t features = kVariant[v].features / (gated ? 2 : 1);
+    const int64_t tiles = (N + features - 1) / features * ((M + kVariant[v].tokens - 1) / kVariant[v].tokens);
+    for (int64_t S = 1; S <= std::min<int64_t>(max_parts, 16) && (S == 1 || steps / S >= 2); S++) {
+      const int64_t each = (steps + S - 1) / S, parts = (steps + each - 1) / each;
+      const double per_cu = std::max(0.5, (double)(tiles * parts) / (double)cus);
+      double us = 3.0 + (double)each * (kVariant[v].one + kVariant[v].more * per_cu);
+      if (parts > 1) us += (own_sum ? 2.2 : 0.0) + (double)(2 * parts + 1) * (double)M * (double)N * 4.0 / 5e6;
+      if (us < best.us) best = MxPlan{v, (int)parts, us};
     }
-    sum = fmaf(p, mx_scale(sw[n * nb + b]), sum);
   }
-  sum = wave_sum(sum);
-  if (lane == 0) y[n] = sum;
+  return best;
 }
 
-static int check_product(const char* who, const void* a, const void* sa, const void* W, const void* sw, const void* out, int64_t M, int64_t N,
-                         int64_t K) {
-  if (!a || !sa || !W || !sw || !out) return fail(TLHIP_EINVAL, "%s: null pointer", who);
-  if (M <= 0 || N <= 0 || !mx_row(K)) return fail(TLHIP_EINVAL, "%s: need M, N > 0, K a positive multiple of 32", who);
-  if (!aligned16(a) || !aligned16(W) || !aligned16(out)) return fail(TLHIP_EINVAL, "%s: elements and result must be 16-byte aligned", who);
-  if (M > (1 << 20) || N > (1 << 24) || K > (1 << 20)) return fail(TLHIP_EUNSUPPORTED, "%s: M, K up to 2^20, N up to 2^24", who);
-  return TLHIP_OK;
+static hipError_t launch_plan(const MxPlan& P, const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N,
+                              int64_t K, float* C, uint8_t* codes, uint8_t* scales) {
+  if (codes) {
+    const auto go = P.variant == 0 ? launch_tiles<1, 4, 8, 1, 4, true> : P.variant == 1 ? launch_tiles<1, 4, 8, 2, 3, true> : launch_tiles<2, 2, 8, 4, 2, true>;
+    return go(A, sa, W, sw, M, N, K, 1, C, codes, scales);
+  }
+  const auto go = P.variant == 0 ? launch_tiles<1, 4, 8, 1, 4, false> : P.variant == 1 ? launch_tiles<1, 4, 8, 2, 3, false> : launch_tiles<2, 2, 8, 4, 2, false>;
+  return go(A, sa, W, sw, M, N, K, P.parts, C, nullptr, nullptr);
 }
 
 }  // namespace tlhip
 
 using namespace tlhip;
 
-extern "C" {
+static const uint8_t* bytes(const void* p) { return static_cast<const uint8_t*>(p); }
 
-int tlhip_gemv_mxfp4(const void* a, const void* codes, const void* scales, void* y, int64_t N, int64_t K) {
-  TLHIP_REQUIRE_READY();
-  if (const int rc = check_product("tlhip_gemv_mxfp4", a, scales, codes, scales, y, 1, N, K)) return rc;
-  mx_gemv_simple_kernel<<<dim3((unsigned)((N + 3) / 4)), dim3(256), 0, ctx().stream>>>(
-      static_cast<const float*>(a), static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<float*>(y), (int)N,
-      (int)(K / 32));
-  TLHIP_CHECK_LAUNCH(TLHIP_C_GEMV_MXFP4);
-}
+extern "C" {
 
 int tlhip_gemm_mxfp4_nt_parts(const void* acodes, const void* ascales, const void* codes, const void* scales, void* parts, int64_t parts_bytes,
                               int64_t M, int64_t N, int64_t K, int* n_parts) {
   TLHIP_REQUIRE_READY();
   const char* who = "tlhip_gemm_mxfp4_nt_parts";
-  if (const int rc = check_product(who, acodes, ascales, codes, scales, parts, M, N, K)) return rc;
+  if (const int rc = check_mx_product(who, acodes, ascales, codes, scales, parts, M, N, K)) return rc;
   if (!n_parts) return fail(TLHIP_EINVAL, "%s: null pointer", who);
   if (parts_bytes < M * N * 4) return fail(TLHIP_EINVAL, "%s: the parts need M * N * 4 bytes at least", who);
-  mx_gemm_simple_kernel<<<dim3((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16)), dim3(64), 0, ctx().stream>>>(
-      static_cast<const uint8_t*>(acodes), static_cast<const uint8_t*>(ascales), static_cast<const uint8_t*>(codes),
-      static_cast<const uint8_t*>(scales), static_cast<float*>(parts), (int)M, (int)N, (int)(K / 32));
-  *n_parts = 1;
+  hipError_t e;
+  if (M <= kMxFewRows) {
+    *n_parts = 1;
+    e = launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, static_cast<float*>(parts), nullptr, nullptr);
+  } else {
+    // (parts of no whole number of 16 bytes would not be stored as such)
+    const MxPlan P = plan_tiles(M, N, K, N % 4 == 0 ? parts_bytes / (M * N * 4) : 1, false, false);
+    *n_parts = P.parts;
+    e = launch_plan(P, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, static_cast<float*>(parts), nullptr, nullptr);
+  }
+  if (e != hipSuccess) return hip_fail(e, who);
   TLHIP_CHECK_LAUNCH(TLHIP_C_GEMM_MXFP4);
 }
 
 int tlhip_gemm_mxfp4_nt(const void* acodes, const void* ascales, const void* codes, const void* scales, void* C, int64_t M, int64_t N,
                         int64_t K) {
   TLHIP_REQUIRE_READY();
-  if (const int rc = check_product("tlhip_gemm_mxfp4_nt", acodes, ascales, codes, scales, C, M, N, K)) return rc;
-  mx_gemm_simple_kernel<<<dim3((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16)), dim3(64), 0, ctx().stream>>>(
-      static_cast<const uint8_t*>(acodes), static_cast<const uint8_t*>(ascales), static_cast<const uint8_t*>(codes),
-      static_cast<const uint8_t*>(scales), static_cast<float*>(C), (int)M, (int)N, (int)(K / 32));
+  const char* who = "tlhip_gemm_mxfp4_nt";
+  if (const int rc = check_mx_product(who, acodes, ascales, codes, scales, C, M, N, K)) return rc;
+  hipError_t e;
+  if (M <= kMxFewRows) {
+    e = launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, static_cast<float*>(C), nullptr, nullptr);
+  } else {
+    MxPlan P = plan_tiles(M, N, K, N % 4 == 0 ? 16 : 1, false, true);
+    float* out = static_cast<float*>(C);
+    if (P.parts > 1) {
+      out = static_cast<float*>(scratch((size_t)P.parts * M * N * 4));
+      if (!out) {            // (a recording may not grow it)
+        P = plan_tiles(M, N, K, 1, false, true);
+        out = static_cast<float*>(C);
+      }
+    }
+    e = launch_plan(P, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, out, nullptr, nullptr);
+    if (e == hipSuccess && P.parts > 1) launch_part_sum(out, static_cast<float*>(C), M, N, N, N, P.parts, 0);
+  }
+  if (e != hipSuccess) return hip_fail(e, who);
   TLHIP_CHECK_LAUNCH(TLHIP_C_GEMM_MXFP4);
 }
 
@@ -197,12 +282,15 @@ int tlhip_gemm_mxfp4_nt_swiglu(const void* acodes, const void* ascales, const vo
                                void* act_scales, int64_t M, int64_t ff, int64_t K) {
   TLHIP_REQUIRE_READY();
   const char* who = "tlhip_gemm_mxfp4_nt_swiglu";
-  if (const int rc = check_product(who, acodes, ascales, codes, scales, act_codes, M, ff, K)) return rc;
+  if (const int rc = check_mx_product(who, acodes, ascales, codes, scales, act_codes, M, ff, K)) return rc;
   if (!act_scales) return fail(TLHIP_EINVAL, "%s: null pointer", who);
   if (!mx_row(ff)) return fail(TLHIP_EINVAL, "%s: ff must be a multiple of 32", who);
-  mx_gated_simple_kernel<<<dim3((unsigned)(ff / 32), (unsigned)((M + 15) / 16)), dim3(64), 0, ctx().stream>>>(
-      static_cast<const uint8_t*>(acodes), static_cast<const uint8_t*>(ascales), static_cast<const uint8_t*>(codes),
-      static_cast<const uint8_t*>(scales), static_cast<uint8_t*>(act_codes), static_cast<uint8_t*>(act_scales), (int)M, (int)ff, (int)(K / 32));
+  uint8_t *qc = static_cast<uint8_t*>(act_codes), *qs = static_cast<uint8_t*>(act_scales);
+  const hipError_t e = M <= kMxFewRows && mx_few_rows_fit(ff, K, true)
+                           ? launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, ff, K, nullptr, qc, qs)
+                           : launch_plan(plan_tiles(M, ff, K, 1, true, false), bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, ff, K,
+                                         nullptr, qc, qs);
+  if (e != hipSuccess) return hip_fail(e, who);
   TLHIP_CHECK_LAUNCH(TLHIP_C_GEMM_MXFP4);
 }
 

@@ -1,0 +1,539 @@
+// Products of few rows over MXFP4 weights: of one f32 row (a decode step's, plain or behind an RMS norm, with or without the gated
+// activation) and of up to 16 MXFP8 rows. All of it is bound by reading the weight.
+#include "mx_mfma.hpp"
+
+#include <algorithm>
+
+namespace tlhip {
+
+// The weight is read once, from memory straight into the registers that the matrix instruction takes it from: a wavefront has 16 NF
+// of its rows and every KW-th unit of 256 k (128 bytes of a row). KW wavefronts of a block share rows; their sums are joined in
+// LDS, in their order. Features that are left over are the last row's again, and not stored.
+//
+// kCodes: up to 16 NT rows of MXFP8, read by every block, in two parts each (above).
+// kFloat, kNormed: one f32 row (kNormed: rms-normed first), cut into digits that the matrix cores multiply exactly. A number's magnitude,
+// over the power of two of its block's largest, is a whole number of 48 bits: twelve digits of four. A byte 0 to 15 is,
+// as e4m3, that many times 2^-9, so a digit is its own code; with the number's sign it is one element of a row of the second operand,
+// digit p in row p under the scale 16^p. The row's twelve sums, which no product's last bit is missing from, are added up at the end. A
+// number keeps all of its 24 bits down to 2^-24 of its block's largest, below that an absolute error of 2^-48 of it. Numbers
+// below 2^-81 are cut at 2^-128; a block with an infinity or a NaN is NaN. Dequantised in the vector unit (1.5 instructions for each
+// weight, the conversion of e2m1 alone nearly three times an FMA) the same product was bound by it.
+//
+// The scales of a block's rows are one run of bytes: copied into LDS whole (a byte loaded by each lane was a request for 16 lines: 70 us
+// instead of 60 over 152064 x 3584).
+typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(1)));
+__device__ __forceinline__ void put_scales(char* to, const uint8_t* from, int bytes, int64_t limit, int tid, int threads) {
+  for (int i = 16 * tid; i < bytes; i += 16 * threads) {
+    if (i + 16 <= limit)
+      *reinterpret_cast<frag16*>(to + i) = *reinterpret_cast<const any16*>(from + i);
+    else
+      for (int k = 0; k < 16 && i + k < limit; k++) to[i + k] = (char)from[i + k];
+  }
+}
+enum { kCodes = 0, kFloat = 1, kNormed = 2 };
+struct MxRow {               // the f32 row: x (+ delta), its norm weights, and where x + delta goes
+  const float *x, *delta, *norm_w;
+  float* xout;
+  float eps;
+};
+constexpr int kDigits = 12, kUnitLds = 2 * kDigits * 128 + 16;      // digits of a unit, its eight blocks' exponents
+
+// Numbers 4 lane .. 4 lane + 3 of a unit into LDS: a step's digits [kDigits][128] bytes, then the next one's, then the exponents
+__device__ __forceinline__ void put_digits(char* lds, int lane, float4 x) {
+  const float v[4] = {x.x, x.y, x.z, x.w};
+  uint32_t big = max(max(magnitude(v[0]), magnitude(v[1])), max(magnitude(v[2]), magnitude(v[3])));
+  big = max(big, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)big, 0xB1, 0xf, 0xf, true));    // quad_perm [1,0,3,2]
+  big = max(big, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)big, 0x4E, 0xf, 0xf, true));    // quad_perm [2,3,0,1]
+  big = max(big, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)big, 0x141, 0xf, 0xf, true));   // row_half_mirror
+  const uint32_t field = max(big >> 23, 46u);
+  const float up1 = __uint_as_float((254u - min(field, 253u)) << 23), up2 = field >= 254u ? 1073741824.0f : 2147483648.0f;
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float a = fabsf(v[i]) * up1 * up2;                 // below 2^32: 2^31 over the largest's power of two
+    hi[i] = (uint32_t)a;                                     // (towards zero; a whole number from 2^24 on)
+    lo[i] = (uint32_t)((a - (float)hi[i]) * 65536.0f);
+  }
+  // byte b of the four numbers in one word
+  const auto plane = [](const uint32_t (&d)[4], int b) {
+    const uint32_t s = 0x0c0c0400u + (uint32_t)b * 0x0101u;  // bytes b of a pair, then zeros
+    return __builtin_amdgcn_perm(d[1], d[0], s) | __builtin_amdgcn_perm(d[3], d[2], s) << 16;
+  };
+  const uint32_t f[4] = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+  const uint32_t sign = plane(f, 3) & 0x80808080u;
+  uint32_t* at = reinterpret_cast<uint32_t*>(lds + (lane >> 5) * (kDigits * 128) + (lane & 31) * 4);
+#pragma unroll
+  for (int b = 0; b < 6; b++) {
+    const uint32_t w = b < 2 ? plane(lo, b) : plane(hi, b - 2);
+    at[(2 * b) * 32] = (w & 0x0f0f0f0fu) | sign;
+    at[(2 * b + 1) * 32] = (w >> 4 & 0x0f0f0f0fu) | sign;
+  }
+  if ((lane & 7) == 0) reinterpret_cast<uint8_t*>(lds + 2 * kDigits * 128)[lane >> 3] = (uint8_t)min(field, 255u);
+}
+
+__host__ __device__ constexpr int rows_sums(int tiles, int waves) { return waves * (tiles * 1024 + 4); }
+
+// The sums of a feature's twelve digits, which lie in lanes 0 .. 11 of the sixteen that have it: lane i gets feature i of its four
+__device__ __forceinline__ float join_digits(const v4f& c, int r) {
+  float mine = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    float v = r < kDigits ? c[i] : 0.f;
+    v = dpp_add_f32<0xB1>(v);
+    v = dpp_add_f32<0x4E>(v);
+    v = dpp_add_f32<0x141>(v);
+    v = dpp_add_f32<0x140>(v);
+    mine = r == i ? v : mine;
+  }
+  return mine * 256.0f;
+}
+
+template <int SRC, int NF, bool GATED>
+__global__ __launch_bounds__(SRC == kCodes ? 512 : 1024, 2) void mx_rows_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ sa,
+                                                         const uint8_t* __restrict__ W, const uint8_t* __restrict__ sw, int M, int N, int nb, int KW,
+                                                         int waves, float* __restrict__ C, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                         const MxRow R) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), fw = wave / KW, kw = wave - fw * KW, FW = waves / KW;
+  const int units = (nb + 7) / 8, K = nb * kMxBlock;
+  constexpr int kTile = GATED ? 8 * NF : 16 * NF;              // features of a wavefront
+  const int n0 = (blockIdx.x * FW + fw) * kTile;
+  const uint8_t* wrow[NF];
+  int wscale[NF];                                              // in the block's run of scales: gate rows first
+#pragma unroll
+  for (int f = 0; f < NF; f++) {
+    const int n = min(n0 + 16 * (GATED ? f % (NF / 2) : f) + r, N - 1);
+    const bool up = GATED && f >= NF / 2;
+    wrow[f] = W + ((up ? (int64_t)N : 0) + n) * nb * 16;
+    wscale[f] = (fw * kTile + 16 * (GATED ? f % (NF / 2) : f) + r + (up ? FW * kTile : 0)) * nb;
+  }
+  const uint8_t *arow = A + (int64_t)min(r, M - 1) * nb * 32, *ascale = sa + (int64_t)min(r, M - 1) * nb;
+  struct Unit {
+    frag16 w[2][NF];
+    frag16 lo[2], hi[2];
+    uint32_t as[2];
+    float4 x, d, nw;
+  };
+  // Past the end of a row: its last block or numbers again, under scales of 2^-127 on both sides (digits: as zeros)
+  const auto ask = [&](Unit& q, int u) {
+    if constexpr (SRC != kCodes) {
+      const int k = min(256 * u + 4 * lane, K - 4);
+      q.x = *reinterpret_cast<const float4*>(R.x + k);
+      if constexpr (SRC == kNormed) {
+        if (R.delta) q.d = *reinterpret_cast<const float4*>(R.delta + k);
+        q.nw = *reinterpret_cast<const float4*>(R.norm_w + k);
+      }
+    }
+    // (both halves of a row's 128 bytes one after the other, and not past the caches: the second finds the line there)
+#pragma unroll
+    for (int f = 0; f < NF; f++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) q.w[h][f] = *reinterpret_cast<const frag16*>(wrow[f] + (int64_t)min(8 * u + 4 * h + g, nb - 1) * 16);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int b = 8 * u + 4 * h + g, at = min(b, nb - 1);
+      if constexpr (SRC == kCodes) {
+        const int c0 = min(16 * u + 8 * h + g, 2 * nb - 1), c1 = min(16 * u + 8 * h + 4 + g, 2 * nb - 1);
+        q.lo[h] = *reinterpret_cast<const frag16*>(arow + (int64_t)c0 * 16);
+        q.hi[h] = *reinterpret_cast<const frag16*>(arow + (int64_t)c1 * 16);
+        q.as[h] = b < nb ? ascale[at] : 0;
+      }
+    }
+  };
+  v4f c[NF];
+#pragma unroll
+  for (int f = 0; f < NF; f++) c[f] = v4f{0.f, 0.f, 0.f, 0.f};
+  float ss = 0.f;
+  char* const mine = lds + wave * kUnitLds;
+  const uint8_t* const run = reinterpret_cast<const uint8_t*>(lds) + (SRC == kCodes ? rows_sums(NF, waves) : max(rows_sums(NF, waves), waves * kUnitLds));
+  const auto multiply = [&](Unit& q, int u) {
+    if constexpr (SRC != kCodes) {
+      const bool live = 256 * u + 4 * lane < K;
+      float4 x = q.x;
+      if constexpr (SRC == kNormed) {
+        if (R.delta) x = plus(x, q.d);
+        if (live && R.xout && blockIdx.x == 0 && fw == 0) *reinterpret_cast<float4*>(R.xout + 256 * u + 4 * lane) = x;
+        ss += live ? (x.x * x.x + x.y * x.y) + (x.z * x.z + x.w * x.w) : 0.f;
+        x.x *= q.nw.x; x.y *= q.nw.y; x.z *= q.nw.z; x.w *= q.nw.w;
+      }
+      if (!live) x = make_float4(0.f, 0.f, 0.f, 0.f);
+      asm volatile("" ::: "memory");                           // (the unit before has been read, in LDS's order)
+      put_digits(mine, lane, x);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int b = 8 * u + 4 * h + g;
+      int ws[NF];
+#pragma unroll
+      for (int f = 0; f < NF; f++) ws[f] = b < nb ? run[wscale[f] + b] : 0;
+      if constexpr (SRC == kCodes) {
+        v8i large, small;
+        split_e4m3(row_operand(q.lo[h], q.hi[h]), large, small);
+#pragma unroll
+        for (int f = 0; f < NF; f++) {
+          c[f] = mx_mma(weight_operand(q.w[h][f]), small, c[f], ws[f], (int)q.as[h]);
+          c[f] = mx_mma(weight_operand(q.w[h][f]), large, c[f], ws[f], (int)q.as[h]);
+        }
+      } else {
+        const int row = min(r, kDigits - 1);
+        const char* s = mine + h * (kDigits * 128) + row * 128 + 16 * g;
+        const frag16 lo = *reinterpret_cast<const frag16*>(s), hi = *reinterpret_cast<const frag16*>(s + 64);
+        const int field = reinterpret_cast<const uint8_t*>(mine + 2 * kDigits * 128)[4 * h + g];
+        const int scale = field == 255 ? 255 : field - 46 + 4 * row;
+        const v8i a = row_operand(lo, hi);
+#pragma unroll
+        for (int f = 0; f < NF; f++) c[f] = mx_mma(weight_operand(q.w[h][f]), a, c[f], ws[f], scale);
+      }
+    }
+  };
+  Unit one, two;
+  if (kw < units) ask(one, kw);
+  {
+    const int rows = FW * kTile, bytes = rows * nb, first = (int)blockIdx.x * rows;
+    char* const to = lds + (reinterpret_cast<const char*>(run) - lds);
+    const int64_t left = (int64_t)(N - first) * nb;
+    put_scales(to, sw + (int64_t)first * nb, bytes, left, tid, 64 * waves);
+    if (GATED) put_scales(to + bytes, sw + ((int64_t)N + first) * nb, bytes, left, tid, 64 * waves);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+  for (int u = kw; u < units; u += 2 * KW) {
+    if (u + KW < units) ask(two, u + KW);
+    multiply(one, u);
+    if (u + KW < units) {
+      if (u + 2 * KW < units) ask(one, u + 2 * KW);
+      multiply(two, u + KW);
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < NF; f++) mx_done(c[f]);
+
+  // the KW wavefronts' sums, added up in their order: tile f by wavefront f % KW, a gated product's all by the first
+  float inv = 1.f;
+  const auto my_tile = [&](int f) { return GATED ? kw == 0 : f % KW == kw; };
+  if (KW > 1 || SRC == kNormed) {
+    __syncthreads();
+    char* const sums = lds + fw * (KW * NF) * 1024;
+    float* const squares = reinterpret_cast<float*>(lds + waves * NF * 1024);
+#pragma unroll
+    for (int f = 0; f < NF; f++) *reinterpret_cast<v4f*>(sums + (f * KW + kw) * 1024 + lane * 16) = c[f];
+    if constexpr (SRC == kNormed) {
+      ss = wave_sum(ss);
+      if (lane == 0) squares[wave] = ss;
+    }
+    __syncthreads();
+    if constexpr (SRC == kNormed) {
+      float total = 0.f;
+      for (int k = 0; k < KW; k++) total += squares[fw * KW + k];
+      inv = 1.0f / sqrtf(total / (float)K + R.eps);
+    }
+#pragma unroll
+    for (int f = 0; f < NF; f++) {
+      if (!my_tile(f)) continue;
+      v4f v = *reinterpret_cast<const v4f*>(sums + f * KW * 1024 + lane * 16);
+      for (int k = 1; k < KW; k++) v += *reinterpret_cast<const v4f*>(sums + (f * KW + k) * 1024 + lane * 16);
+      c[f] = v;
+    }
+  }
+  if constexpr (SRC != kCodes) {
+    // a digit's sums lie in one lane of a row of 16; lane i < 4 of them stores feature 4 g + i
+    float out[NF];
+#pragma unroll
+    for (int f = 0; f < NF; f++)
+      if (my_tile(f)) out[f] = join_digits(c[f], r) * inv;
+    const int n = n0 + 4 * g + r;
+    if constexpr (GATED) {
+#pragma unroll
+      for (int f = 0; f < NF / 2; f++)
+        if (kw == 0 && r < 4 && n + 16 * f < N) C[n + 16 * f] = gated(out[f], out[f + NF / 2]);
+    } else {
+#pragma unroll
+      for (int f = 0; f < NF; f++)
+        if (my_tile(f) && r < 4 && n + 16 * f < N) C[n + 16 * f] = out[f];
+    }
+  } else if constexpr (GATED) {
+    if (kw != 0) return;
+#pragma unroll
+    for (int p = 0; p < NF / 4; p++) {
+      const int n = n0 + 32 * p;
+      const int64_t m = min(r, M - 1);
+      store_gated(c[2 * p], c[2 * p + 1], c[NF / 2 + 2 * p], c[NF / 2 + 2 * p + 1], g, r < M && n < N, codes + m * N + n,
+                  scales + m * (N / kMxBlock) + n / kMxBlock);
+    }
+  } else {
+#pragma unroll
+    for (int f = 0; f < NF; f++)
+      if (my_tile(f) && r < M) store_features(C + (int64_t)r * N, n0 + 16 * f + 4 * g, N, c[f]);
+  }
+}
+
+template <int SRC, int NF, bool GATED>
+static hipError_t launch_rows(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N, int64_t K, int KW,
+                              int waves, float* C, uint8_t* codes, uint8_t* scales, const MxRow& R) {
+  constexpr int kTile = GATED ? 8 * NF : 16 * NF;
+  const int lds = std::max(SRC == kCodes ? 0 : waves * kUnitLds, rows_sums(NF, waves)) + (int)(waves / KW * 16 * NF * (K / kMxBlock)) + 16;
+  const auto kernel = mx_rows_kernel<SRC, NF, GATED>;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+  if (e != hipSuccess) return e;
+  const int64_t per_block = (int64_t)kTile * (waves / KW);
+  kernel<<<dim3((unsigned)((N + per_block - 1) / per_block)), dim3(64 * waves), lds, ctx().stream>>>(
+      A, sa, W, sw, (int)M, (int)N, (int)(K / kMxBlock), KW, waves, C, codes, scales, R);
+  return hipGetLastError();
+}
+
+// The same product where a block has several tiles' worth of rows: the digits of the row, which every tile meets, stay in LDS, the next
+// tile's weights and scales are asked for while this one is multiplied, and blocks walk the tiles without a break. UPW:
+// units of 256 k a wavefront has (K up to 256 KW UPW).
+template <int SRC, int NF, bool GATED, int UPW>
+__global__ __launch_bounds__(512, UPW * NF <= 4 ? 4 : 2) void mx_row_tiles_kernel(const uint8_t* __restrict__ W, const uint8_t* __restrict__ sw, int N, int nb, int KW,
+                                                              int tiles, float* __restrict__ y, const MxRow R) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), fw = wave / KW, kw = wave - fw * KW, FW = 8 / KW;
+  const int K = nb * kMxBlock;
+  constexpr int kTile = GATED ? 8 * NF : 16 * NF, kDigitLds = 8 * UPW * kUnitLds;
+  const int rows = FW * kTile, run_bytes = rows * nb, run_stage = ((GATED ? 2 : 1) * run_bytes + 15) & ~15;
+  char* const mine = lds + wave * UPW * kUnitLds;
+  char* const runs = lds + kDigitLds;
+  float* const sums = reinterpret_cast<float*>(runs + 2 * run_stage);      // [2][8 wavefronts][NF][16]
+  float* const squares = sums + 2 * 8 * NF * 16;
+  frag16 q[UPW][2][NF];
+  const uint8_t* row[NF];
+  const auto rows_of = [&](int tile) {
+    const int n0 = min(tile, tiles - 1) * rows + fw * kTile;
+#pragma unroll
+    for (int f = 0; f < NF; f++) {
+      const int n = min(n0 + 16 * (GATED ? f % (NF / 2) : f) + r, N - 1);
+      row[f] = W + ((GATED && f >= NF / 2 ? (int64_t)N : 0) + n) * nb * 16;
+    }
+  };
+  // (both halves of a row's 128 bytes one after the other, and not past the caches: the second finds the line there)
+  const auto ask = [&](int j, int f) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) q[j][h][f] = *reinterpret_cast<const frag16*>(row[f] + (uint32_t)min(8 * (kw + j * KW) + 4 * h + g, nb - 1) * 16u);
+  };
+  const auto ask_all = [&](int tile) {
+    rows_of(tile);
+#pragma unroll
+    for (int j = 0; j < UPW; j++)
+#pragma unroll
+      for (int f = 0; f < NF; f++) ask(j, f);
+  };
+  // scales of a tile, 16 bytes a thread (the launcher sees to it that the run is no more than 512 of those, and whole ones)
+  any16 sc[GATED ? 2 : 1];
+  const auto ask_scales = [&](int tile) {
+    const int64_t total = (int64_t)N * nb, at = min((int64_t)min(tile, tiles - 1) * run_bytes + min(16 * tid, run_bytes - 16), total - 16);
+#pragma unroll
+    for (int k = 0; k < (GATED ? 2 : 1); k++) sc[k] = *reinterpret_cast<const any16*>(sw + k * total + at);
+  };
+  const auto keep_scales = [&](int stage) {
+#pragma unroll
+    for (int k = 0; k < (GATED ? 2 : 1); k++)
+      if (16 * tid < run_bytes) *reinterpret_cast<frag16*>(runs + stage * run_stage + k * run_bytes + 16 * tid) = sc[k];
+  };
+  int tile = blockIdx.x;
+  // my units of the row, its digits kept; squares are of the row before the norm's weights
+  float4 x[UPW], d[UPW], nw[UPW];
+#pragma unroll
+  for (int j = 0; j < UPW; j++) {
+    const int k = min(256 * (kw + j * KW) + 4 * lane, K - 4);
+    x[j] = *reinterpret_cast<const float4*>(R.x + k);
+    if constexpr (SRC == kNormed) {
+      d[j] = R.delta ? *reinterpret_cast<const float4*>(R.delta + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+      nw[j] = *reinterpret_cast<const float4*>(R.norm_w + k);
+    }
+  }
+  ask_scales(tile);
+  if (UPW * NF <= 2) ask_all(tile);               // (more than a unit's weights beside the digits' numbers do not fit the registers)
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < UPW; j++) {
+    const int k = 256 * (kw + j * KW) + 4 * lane;
+    float4 v = x[j];
+    if constexpr (SRC == kNormed) {
+      if (R.delta) v = plus(v, d[j]);
+      if (k < K && R.xout && blockIdx.x == 0 && fw == 0) *reinterpret_cast<float4*>(R.xout + k) = v;
+      ss += k < K ? (v.x * v.x + v.y * v.y) + (v.z * v.z + v.w * v.w) : 0.f;
+      v.x *= nw[j].x; v.y *= nw[j].y; v.z *= nw[j].z; v.w *= nw[j].w;
+    }
+    if (k >= K) v = make_float4(0.f, 0.f, 0.f, 0.f);
+    put_digits(mine + j * kUnitLds, lane, v);
+  }
+  if (UPW * NF > 2) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    ask_all(tile);
+  }
+  if constexpr (SRC == kNormed) {
+    ss = wave_sum(ss);
+    if (lane == 0) squares[wave] = ss;
+  }
+  keep_scales(0);
+  float inv = 1.f;
+  const int digit = min(r, kDigits - 1);
+  const auto meet = [] {          // LDS writes only: what is asked for stays in flight
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  meet();
+  if constexpr (SRC == kNormed) {
+    float total = 0.f;
+    for (int k = 0; k < KW; k++) total += squares[fw * KW + k];
+    inv = 1.0f / sqrtf(total / (float)K + R.eps);
+  }
+  for (int stage = 0; tile < tiles; stage ^= 1) {
+    const int next = tile + (int)gridDim.x;
+    ask_scales(next);
+    rows_of(next);
+    const uint8_t* run = reinterpret_cast<const uint8_t*>(runs) + stage * run_stage;
+    v4f c[NF];
+#pragma unroll
+    for (int f = 0; f < NF; f++) c[f] = v4f{0.f, 0.f, 0.f, 0.f};
+    // a register that has been multiplied is asked for again: the next tile's weights
+#pragma unroll
+    for (int j = 0; j < UPW; j++) {
+      v8i a[2];
+      int scale[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const char* s = mine + j * kUnitLds + h * (kDigits * 128) + digit * 128 + 16 * g;
+        const frag16 lo = *reinterpret_cast<const frag16*>(s), hi = *reinterpret_cast<const frag16*>(s + 64);
+        const int field = reinterpret_cast<const uint8_t*>(mine + j * kUnitLds + 2 * kDigits * 128)[4 * h + g];
+        scale[h] = field == 255 ? 255 : field - 46 + 4 * digit;
+        a[h] = row_operand(lo, hi);
+      }
+#pragma unroll
+      for (int f = 0; f < NF; f++) {
+        const int in_run = (GATED && f >= NF / 2 ? run_bytes : 0) + (fw * kTile + 16 * (GATED ? f % (NF / 2) : f) + r) * nb;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int b = 8 * (kw + j * KW) + 4 * h + g, ws = b < nb ? run[in_run + b] : 0;
+          c[f] = mx_mma(weight_operand(q[j][h][f]), a[h], c[f], ws, scale[h]);
+        }
+        ask(j, f);
+      }
+    }
+    float* const part = sums + stage * (8 * NF * 16);
+#pragma unroll
+    for (int f = 0; f < NF; f++) {
+      mx_done(c[f]);
+      const float v = join_digits(c[f], r);
+      if (r < 4) part[(wave * NF + f) * 16 + 4 * g + r] = v;
+    }
+    keep_scales(stage ^ 1);
+    meet();
+    // a row's sums over the KW wavefronts, one row a thread
+    if (tid < FW * NF * 16) {
+      const int w = tid / (NF * 16), f = tid / 16 % NF, i = tid & 15;
+      const auto sum = [&](int ff) {
+        float v = part[(w * KW * NF + ff) * 16 + i];
+        for (int k = 1; k < KW; k++) v += part[((w * KW + k) * NF + ff) * 16 + i];
+        return v * inv;
+      };
+      if constexpr (GATED) {
+        const int n = tile * rows + w * kTile + 16 * f + i;
+        if (f < NF / 2 && n < N) y[n] = gated(sum(f), sum(f + NF / 2));
+      } else {
+        const int n = tile * rows + w * kTile + 16 * f + i;
+        if (n < N) y[n] = sum(f);
+      }
+    }
+    tile = next;
+  }
+}
+
+template <int SRC, int NF, bool GATED, int UPW>
+static hipError_t launch_row_tiles(const uint8_t* W, const uint8_t* sw, int64_t N, int64_t K, int KW, int per_cu, float* y, const MxRow& R) {
+  constexpr int kTile = GATED ? 8 * NF : 16 * NF;
+  const int nb = (int)(K / kMxBlock), rows = 8 / KW * kTile, run = rows * nb, lds = 8 * UPW * kUnitLds + 2 * (((GATED ? 2 : 1) * run + 15) & ~15) + (2 * 8 * NF * 16 + 8) * 4;
+  const int tiles = (int)((N + rows - 1) / rows);
+  const auto kernel = mx_row_tiles_kernel<SRC, NF, GATED, UPW>;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+  if (e != hipSuccess) return e;
+  kernel<<<dim3((unsigned)std::min(tiles, per_cu * cu_count())), dim3(512), lds, ctx().stream>>>(W, sw, (int)N, nb, KW, tiles, y, R);
+  return hipGetLastError();
+}
+
+// Which kernel, by sizes (us so, and in the other forms):
+//   more than 4 tiles of 16 rows for each CU, K up to 4096: mx_row_tiles_kernel (152064 x 3584 51.6, row by row 55.2; 37888 x 3584 14.8, 16.0;
+//     9728 x 896, 2.4 tiles: 4.2, 4.2);
+//   K up to 1024: four wavefronts share a row's K, two sets of them a block (9728 x 896 4.2; eight: 4.4);
+//   up to twelve units of 256 k: eight; beyond: sixteen (3584 x 18944 9.8; eight 10.8; 4608 x 3584 4.8; 5.2);
+//   32 rows a block from 4096 on, where that still makes more than half as many blocks as there are CUs (4608 x 3584 4.8, 16: 5.3;
+//     3584 x 18944 12.9, 16: 9.8), and while the scales of their rows leave room in LDS.
+template <int SRC, bool GATED>
+static hipError_t launch_row(const uint8_t* W, const uint8_t* sw, int64_t N, int64_t K, float* y, const MxRow& R) {
+  const int64_t nb = K / kMxBlock, units = (nb + 7) / 8, cus = cu_count();
+  const int KW = units <= 4 ? 4 : 8;
+  const int64_t rows = 16 * (8 / KW);          // of a tile, gate rows if gated
+  if (units <= 16 && N % 16 == 0 && N > 4 * cus * rows && rows * nb >= 16) {
+    constexpr int NF = GATED ? 2 : 1;
+    return (units <= KW ? launch_row_tiles<SRC, NF, GATED, 1> : launch_row_tiles<SRC, NF, GATED, 2>)(W, sw, N, K, KW, 2, y, R);
+  }
+  const int waves = units <= 12 ? 8 : 16, kw = units <= 4 ? 4 : waves;
+  if constexpr (GATED) return launch_rows<SRC, 2, true>(nullptr, nullptr, W, sw, 1, N, K, kw, waves, y, nullptr, nullptr, R);
+  else
+    return (N > 16 * cus && nb <= 1024 ? launch_rows<SRC, 2, false> : launch_rows<SRC, 1, false>)(nullptr, nullptr, W, sw, 1, N, K, kw, waves, y, nullptr,
+                                                                                               nullptr, R);
+}
+
+bool mx_few_rows_fit(int64_t N, int64_t K, bool gated) {
+  // (a gated block has the scales of 64 rows in LDS beside 32 KB of sums)
+  return !gated || 64 * (K / kMxBlock) <= 120 * 1024;
+}
+hipError_t launch_mx_few_rows(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N, int64_t K, float* C,
+                              uint8_t* codes, uint8_t* scales) {
+  if (codes) return launch_rows<kCodes, 4, true>(A, sa, W, sw, M, N, K, 8, 8, C, codes, scales, MxRow{});
+  return (N > 16 * cu_count() && K <= 32768 ? launch_rows<kCodes, 2, false> : launch_rows<kCodes, 1, false>)(A, sa, W, sw, M, N, K, 8, 8, C, nullptr,
+                                                                                                       nullptr, MxRow{});
+}
+
+}  // namespace tlhip
+
+using namespace tlhip;
+
+static const uint8_t* bytes(const void* p) { return static_cast<const uint8_t*>(p); }
+
+extern "C" {
+
+int tlhip_gemv_mxfp4(const void* a, const void* codes, const void* scales, void* y, int64_t N, int64_t K) {
+  TLHIP_REQUIRE_READY();
+  const char* who = "tlhip_gemv_mxfp4";
+  if (const int rc = check_mx_product(who, a, scales, codes, scales, y, 1, N, K)) return rc;
+  const MxRow R{static_cast<const float*>(a), nullptr, nullptr, nullptr, 0.f};
+  const hipError_t e = launch_row<kFloat, false>(bytes(codes), bytes(scales), N, K, static_cast<float*>(y), R);
+  if (e != hipSuccess) return hip_fail(e, who);
+  TLHIP_CHECK_LAUNCH(TLHIP_C_GEMV_MXFP4);
+}
+
+static int normed(const char* who, const void* x, const void* delta, const void* norm_w, void* xout, const void* codes, const void* scales, void* y,
+                  int64_t N, int64_t K, float eps, bool gate) {
+  if (const int rc = check_mx_product(who, x, scales, codes, scales, y, 1, N, K)) return rc;
+  if (!norm_w) return fail(TLHIP_EINVAL, "%s: null pointer", who);
+  if (!aligned16(delta) || !aligned16(norm_w) || !aligned16(xout)) return fail(TLHIP_EINVAL, "%s: delta, norm_w and xout must be 16-byte aligned", who);
+  if (xout && (xout == x || xout == delta)) return fail(TLHIP_EINVAL, "%s: xout must not alias x or delta", who);
+  const MxRow R{static_cast<const float*>(x), static_cast<const float*>(delta), static_cast<const float*>(norm_w), static_cast<float*>(xout), eps};
+  const hipError_t e = (gate ? launch_row<kNormed, true> : launch_row<kNormed, false>)(bytes(codes), bytes(scales), N, K, static_cast<float*>(y), R);
+  if (e != hipSuccess) return hip_fail(e, who);
+  TLHIP_CHECK_LAUNCH(TLHIP_C_GEMV_MXFP4);
+}
+
+int tlhip_gemv_mxfp4_rmsnorm(const void* x, const void* delta, const void* norm_w, void* xout, const void* codes, const void* scales, void* y,
+                             int64_t N, int64_t K, float eps) {
+  TLHIP_REQUIRE_READY();
+  return normed("tlhip_gemv_mxfp4_rmsnorm", x, delta, norm_w, xout, codes, scales, y, N, K, eps, false);
+}
+
+int tlhip_gemv_mxfp4_rmsnorm_gateup(const void* x, const void* delta, const void* norm_w, void* xout, const void* codes, const void* scales, void* act,
+                                    int64_t N2, int64_t K, float eps) {
+  TLHIP_REQUIRE_READY();
+  const char* who = "tlhip_gemv_mxfp4_rmsnorm_gateup";
+  if (N2 % 2) return fail(TLHIP_EINVAL, "%s: need as many gate rows as up rows", who);
+  return normed(who, x, delta, norm_w, xout, codes, scales, act, N2 / 2, K, eps, true);
+}
+
+}  // extern "C"

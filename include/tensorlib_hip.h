@@ -637,7 +637,8 @@ int tlhip_latent_attn_run(const void* u, int64_t ldu, const void* q, int64_t ldq
  * scales [rows][K/32] bytes in both. Rows are dense and K is a multiple of 32, so rows of two matrices of the same K can be stacked.
  * Rounding a block: s = floor(log2(largest magnitude)) + 127 - 2 (MXFP4) or - 8 (MXFP8), at least 0; every element is the value
  * over 2^(s - 127), rounded to nearest, ties to even, magnitudes beyond the type's largest becoming that. A block that holds
- * an infinity or a NaN gets the scale 255 and elements 0. Elements must be 16-byte aligned, scales need no alignment. */
+ * an infinity or a NaN gets the scale 255 and elements 0. Elements must be 16-byte aligned, scales need no alignment. Products take
+ * M up to 2^20, N up to 2^24 and K up to 65536. */
 /* rows of TLHIP_T_F32, _F16 or _BF16 as a model file holds them -> MXFP4 */
 int tlhip_quantize_mxfp4(const void* src, int src_type, void* codes, void* scales, int64_t rows, int64_t K);
 /* f32 rows -> MXFP8 */
@@ -650,8 +651,14 @@ int tlhip_dequantize_mxfp8(const void* codes, const void* scales, void* dst, int
  * n up to 32768, S up to 64. A row's bytes do not depend on how many rows there are. */
 int tlhip_rmsnorm_res_mxfp8(const void* x, const void* parts, int64_t S, const void* w, void* xout, void* codes, void* scales,
                             int64_t n, float eps, int64_t rows);
-/* y[n] = sum_k a[k] W[n][k], a f32, W MXFP4 [N][K], f32 sums: the decode product. */
+/* y[n] = sum_k a[k] W[n][k], a f32, W MXFP4 [N][K], f32 sums: the decode product. A number of a keeps its 24 bits down to 2^-24 of the
+ * largest of its block of 32, below that an absolute error of 2^-48 of that (and of 2^-128); an infinity or a NaN in a makes every y NaN. */
 int tlhip_gemv_mxfp4(const void* a, const void* codes, const void* scales, void* y, int64_t N, int64_t K);
+/* The same with the producers of tlhip_gemv_q4_rmsnorm and tlhip_gemv_q4_rmsnorm_gateup, whose arguments these have. */
+int tlhip_gemv_mxfp4_rmsnorm(const void* x, const void* delta, const void* norm_w, void* xout, const void* codes, const void* scales, void* y,
+                             int64_t N, int64_t K, float eps);
+int tlhip_gemv_mxfp4_rmsnorm_gateup(const void* x, const void* delta, const void* norm_w, void* xout, const void* codes, const void* scales,
+                                    void* act, int64_t N2, int64_t K, float eps);
 /* C[M][N] f32 = A . W^T, A MXFP8 [M][K], W MXFP4 [N][K]: products of elements are exact, sums are f32. _parts as
  * tlhip_gemm_bf16_nt_parts. */
 int tlhip_gemm_mxfp4_nt(const void* acodes, const void* ascales, const void* codes, const void* scales, void* C, int64_t M, int64_t N,

@@ -245,7 +245,8 @@ def test_gated_product_to_mxfp8(lib, M, ff, K):
                 mx.values(ac, asc, False), mx.values(wc, wsc, True), K)
 
 
-TOKENS = [(1, 32), (3, 64), (17, 96), (16, 512), (896, 896), (1000, 544), (33, 4896), (896, 4864), (4608, 3584), (257, 18944), (20000, 160)]
+TOKENS = [(1, 32), (3, 64), (17, 96), (16, 512), (896, 896), (1000, 544), (33, 4896), (896, 4864), (4608, 3584), (257, 18944), (20000, 160),
+          (33280, 160), (16640, 3584), (16656, 1184), (16650, 1184), (40, 65536)]
 
 
 @pytest.mark.parametrize("N,K", TOKENS)
@@ -259,6 +260,111 @@ def test_token_product(lib, N, K):
     big = np.abs(x[0].astype(np.float64)).reshape(-1, 32).max(-1).repeat(32)
     bound = product_bound(x.astype(np.float64), w, K)[0] + 2.0 ** -38 * (np.abs(w) @ big)
     assert (np.abs(got - w @ x[0].astype(np.float64)) <= bound).all()
+
+
+@pytest.mark.parametrize("N,K", [(1, 32), (17, 96), (896, 896), (1152, 896), (130, 4896), (4608, 3584), (33280, 160), (16640, 2080), (48, 18944), (40, 65536)])
+@pytest.mark.parametrize("delta", [False, True])
+def test_token_product_behind_a_norm(lib, N, K, delta):
+    """Row totals are multiplied by 1 / rms, whose own error is K / 64 additions a lane and 14 more (2^-24 each, half of it in the root),
+    and the numbers by the norm's weights: two roundings each."""
+    r = rng(20, N, K)
+    x, d, nw, (wc, wsc) = activations(r, 1, K)[0], activations(r, 1, K)[0], (1 + 0.1 * r.standard_normal(K)).astype(np.float32), weight(r, N, K)
+    w, s = mx.values(wc, wsc, True), x + d if delta else x
+    s64 = s.astype(np.float64)
+    h = s64 / np.sqrt((s64 * s64).mean() + EPS) * nw
+    out, xout = guarded(lib, 4 * N), guarded(lib, 4 * K)
+    lib.gemv_mxfp4_rmsnorm(lib.to_device(x), lib.to_device(d) if delta else None, lib.to_device(nw), xout, *upload_rows(lib, wc, wsc, True), out, N, K, EPS)
+    assert np.array_equal(taken(xout, 4 * K, np.float32, (K,)), s)
+    got = taken(out, 4 * N, np.float32, (N,))
+    rel = (K / 64 + 20) * 2.0 ** -24
+    assert (np.abs(got - w @ h) <= product_bound(h[None], w, K)[0] + rel * (np.abs(w) @ np.abs(h))).all()
+
+
+@pytest.mark.parametrize("ff,K", [(1, 32), (17, 96), (896, 896), (4864, 896), (130, 4896), (2432, 3584), (33280, 160), (16640, 2080), (48, 18944), (20, 65536)])
+@pytest.mark.parametrize("delta", [False, True])
+def test_gated_token_product_behind_a_norm(lib, ff, K, delta):
+    r = rng(21, ff, K)
+    x, d, nw, (wc, wsc) = activations(r, 1, K)[0], activations(r, 1, K)[0], (1 + 0.1 * r.standard_normal(K)).astype(np.float32), weight(r, 2 * ff, K)
+    w, s = mx.values(wc, wsc, True), (x + d if delta else x).astype(np.float64)
+    h = s / np.sqrt((s * s).mean() + EPS) * nw
+    out = guarded(lib, 4 * ff)
+    lib.gemv_mxfp4_rmsnorm_gateup(lib.to_device(x), lib.to_device(d) if delta else None, lib.to_device(nw), None, *upload_rows(lib, wc, wsc, True), out,
+                                  2 * ff, K, EPS)
+    got = taken(out, 4 * ff, np.float32, (ff,))
+    gu = w @ h
+    off = product_bound(h[None], w, K)[0] + (K / 64 + 20) * 2.0 ** -24 * (np.abs(w) @ np.abs(h))
+    g, u = gu[:ff], gu[ff:]
+    silu = g / (1 + np.exp(-g))
+    # a gate's slope is below 1.1; eight roundings of the gate's own arithmetic
+    assert (np.abs(got - silu * u) <= 1.1 * np.abs(u) * off[:ff] + np.abs(silu) * off[ff:] + 1.2 * off[:ff] * off[ff:] + np.abs(silu * u) * 2.0 ** -20 + 1e-37).all()
+
+
+def test_token_product_is_that_of_the_rows_apart(lib):
+    """A row of the weight gives the same sum whatever rows lie beside it (blocks of one launch shape)."""
+    r = rng(22)
+    x, (wc, wsc) = lib.to_device(activations(r, 1, 896)), weight(r, 96, 896)
+    whole, part = lib.empty(96), lib.empty(32)
+    lib.gemv_mxfp4(x, *upload_rows(lib, wc, wsc, True), whole, 96, 896)
+    lib.gemv_mxfp4(x, *upload_rows(lib, wc[32:64], wsc[32:64], True), part, 32, 896)
+    assert np.array_equal(whole.numpy()[32:64], part.numpy())
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+@pytest.mark.parametrize("M,K", [(1, 896), (5, 896), (70, 896), (70, 1184)])
+def test_scales_anywhere(lib, M, K, off):
+    """Scale bytes at odd addresses, of both operands: products and the decode product."""
+    r, N = rng(23, M, K), 130
+    (ac, asc), (wc, wsc), x = rows8(r, M, K), weight(r, N, K), activations(r, 1, K)
+    a, w = mx.values(ac, asc, False), mx.values(wc, wsc, True)
+
+    def shifted(scales):
+        b = lib.to_device(np.concatenate([np.full(off, 255, np.uint8), scales.reshape(-1)]))
+        b.ptr += off
+        return b
+    da, dw, sa, sw, out = lib.to_device(ac), lib.to_device(mx.pack(wc)), shifted(asc), shifted(wsc), lib.empty((M, N))
+    lib.gemm_mxfp4_nt(da, sa, dw, sw, out, M, N, K)
+    assert (np.abs(out.numpy() - a @ w.T) <= product_bound(a, w, K)).all()
+    y = lib.empty(N)
+    lib.gemv_mxfp4(lib.to_device(x), dw, sw, y, N, K)
+    big = np.abs(x[0].astype(np.float64)).reshape(-1, 32).max(-1).repeat(32)
+    assert (np.abs(y.numpy() - w @ x[0]) <= product_bound(x.astype(np.float64), w, K)[0] + 2.0 ** -38 * (np.abs(w) @ big)).all()
+    for b in (sa, sw):
+        b.ptr -= off
+
+
+@pytest.mark.parametrize("kind", ["spread", "largest", "smallest", "one outlier"])
+def test_token_product_of_hard_rows(lib, kind):
+    """f32 sums of the row's numbers as they are: magnitudes all over a block, at both ends of f32, and one that dwarfs its
+    neighbours under weights of zero."""
+    r, N, K = rng(24), 64, 1152
+    x, (wc, wsc) = r.standard_normal((1, K)).astype(np.float32), weight(r, N, K)
+    if kind == "spread":
+        x *= 2.0 ** r.integers(-22, 1, (1, K)).astype(np.float32)
+    elif kind == "largest":
+        x *= np.float32(2.0 ** 125) / np.abs(x).max()
+        wsc = (wsc - 8).astype(np.uint8)
+    elif kind == "smallest":
+        x *= np.float32(2.0 ** -100)
+        wsc = (wsc + 20).astype(np.uint8)
+    else:
+        x[0, 5::32] = 2.0 ** 20
+        wc[:, 5::32] &= 8
+    w, x64 = mx.values(wc, wsc, True), x.astype(np.float64)
+    out = lib.empty(N)
+    lib.gemv_mxfp4(lib.to_device(x), *upload_rows(lib, wc, wsc, True), out, N, K)
+    big = np.abs(x64[0]).reshape(-1, 32).max(-1).repeat(32)
+    bound = product_bound(x64, w, K)[0] + np.abs(w) @ np.maximum(2.0 ** -48 * big, 2.0 ** -128)
+    assert (np.abs(out.numpy() - w @ x64[0]) <= bound).all()
+
+
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_token_product_of_a_row_that_is_not_finite(lib, bad):
+    r = rng(25)
+    x, (wc, wsc) = activations(r, 1, 896), weight(r, 100, 896)
+    x[0, 777] = bad
+    out = lib.empty(100)
+    lib.gemv_mxfp4(lib.to_device(x), *upload_rows(lib, wc, wsc, True), out, 100, 896)
+    assert np.isnan(out.numpy()).all()
 
 
 @pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e12, 1e30])
@@ -399,7 +505,12 @@ def test_refusals(lib):
         (c.tlhip_rmsnorm_res_mxfp8, (p, None, 0, p, None, p, p, 32, 1e-6, 0), EINVAL),
         (c.tlhip_gemv_mxfp4, (p, p, p, None, 1, 32), EINVAL), (c.tlhip_gemv_mxfp4, (p, p, p, p, 1, 48), EINVAL),
         (c.tlhip_gemv_mxfp4, (p, odd, p, p, 1, 32), EINVAL), (c.tlhip_gemv_mxfp4, (p, p, p, p, 0, 32), EINVAL),
-        (c.tlhip_gemv_mxfp4, (p, p, p, p, 1 << 40, 32), EUNSUPPORTED),
+        (c.tlhip_gemv_mxfp4, (p, p, p, p, 1 << 40, 32), EUNSUPPORTED), (c.tlhip_gemv_mxfp4, (p, p, p, p, 1, 65568), EUNSUPPORTED),
+        (c.tlhip_gemv_mxfp4_rmsnorm, (p, None, None, None, p, p, p, 1, 32, 1e-6), EINVAL),
+        (c.tlhip_gemv_mxfp4_rmsnorm, (p, odd, p, None, p, p, p, 1, 32, 1e-6), EINVAL),
+        (c.tlhip_gemv_mxfp4_rmsnorm, (p, None, p, p, p, p, p, 1, 32, 1e-6), EINVAL),
+        (c.tlhip_gemv_mxfp4_rmsnorm_gateup, (p, None, p, None, p, p, p, 3, 32, 1e-6), EINVAL),
+        (c.tlhip_gemv_mxfp4_rmsnorm_gateup, (p, None, p, None, p, p, p, 2, 33, 1e-6), EINVAL),
         (c.tlhip_gemm_mxfp4_nt, (p, None, p, p, p, 1, 1, 32), EINVAL), (c.tlhip_gemm_mxfp4_nt, (p, p, p, p, p, 0, 1, 32), EINVAL),
         (c.tlhip_gemm_mxfp4_nt, (p, p, p, p, p, 1, 1, 31), EINVAL), (c.tlhip_gemm_mxfp4_nt, (odd, p, p, p, p, 1, 1, 32), EINVAL),
         (c.tlhip_gemm_mxfp4_nt, (p, p, p, p, p, 1 << 30, 1, 32), EUNSUPPORTED),
