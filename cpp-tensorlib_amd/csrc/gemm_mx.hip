@@ -12,6 +12,10 @@ namespace tlhip {
 // serves together find different banks. A row's four scale bytes of a step are one word, which a lane shifts down to its own block's.
 // WORDS: that word is a whole one in memory, too (K % 128 == 0, so that no step ends past a row); elsewhere it is read
 // from wherever it lies.
+// Bound by the matrix cores: each element is multiplied twice, as its large and its small half, so their ceiling is half the
+// formats' (about 1.9e15 products and sums a second at the clock that such a load leaves). 2048 x 37888 x 3584 with the gate takes
+// 424 us (1.31e15 a second), 512 x 3584 x 18944 66 us (1.05e15, two parts' traffic and their sum in it). The activations straight
+// into registers took 484 us instead of 436; a third stage of LDS and raised wave priorities changed nothing.
 typedef uint32_t any4 __attribute__((aligned(1)));
 __device__ __forceinline__ uint32_t four_scales(const uint8_t* row, int b, int nb) {      // bytes b .. b + 3 of nb, 0 past them (b < nb)
   if (nb < 4) {
@@ -193,7 +197,9 @@ static hipError_t launch_tiles(const uint8_t* A, const uint8_t* sa, const uint8_
 // ---- which tiles --------------------------------------------------------------------------------------------------------
 // Features x tokens of a tile and its blocks on a CU: 128 x 64 (four), 128 x 128 (three), 256 x 128 (two). A step takes `one` us plus
 // `more` for each block on a CU, as measured on products of 30 to 2048 rows by 896 x 4864 to 37888 x 3584; the launch that adds
-// parts up 2.2 us and their traffic at 5 TB/s.
+// parts up 2.2 us and their traffic at 3.5 TB/s. Over 54 products of those sizes (every tile, 1 to 16 parts) the choice takes 1.01
+// times the best one's time in the mean and 1.12 at worst. Both sides: 77 x 896 x 4864 8.7 us in 13 parts of 128 x 64, 23.9 in one;
+// 2048 x 37888 x 3584 in one part 422 us with 256 x 128, 427 with 128 x 128, 532 with 128 x 64.
 struct MxPlan { int variant = 0, parts = 1; double us = 1e30; };
 static const struct { int features, tokens; double one, more; } kVariant[3] = {{128, 64, 0.35, 0.38}, {128, 128, 0.4, 0.72}, {256, 128, 0.9, 1.55}};
 
@@ -207,7 +213,7 @@ static MxPlan plan_tiles(int64_t M, int64_t N, int64_t K, int64_t max_parts, boo
       const int64_t each = (steps + S - 1) / S, parts = (steps + each - 1) / each;
       const double per_cu = std::max(0.5, (double)(tiles * parts) / (double)cus);
       double us = 3.0 + (double)each * (kVariant[v].one + kVariant[v].more * per_cu);
-      if (parts > 1) us += (own_sum ? 2.2 : 0.0) + (double)(2 * parts + 1) * (double)M * (double)N * 4.0 / 5e6;
+      if (parts > 1) us += (own_sum ? 2.2 : 0.0) + (double)(2 * parts + 1) * (double)M * (double)N * 4.0 / 3.5e6;
       if (us < best.us) best = MxPlan{v, (int)parts, us};
     }
   }

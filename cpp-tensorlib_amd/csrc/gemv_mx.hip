@@ -461,20 +461,21 @@ static hipError_t launch_row_tiles(const uint8_t* W, const uint8_t* sw, int64_t 
 // Which kernel, by sizes (us so, and in the other forms):
 //   more than 4 tiles of 16 rows for each CU, K up to 4096: mx_row_tiles_kernel (152064 x 3584 51.6, row by row 55.2; 37888 x 3584 14.8, 16.0;
 //     9728 x 896, 2.4 tiles: 4.2, 4.2);
-//   K up to 1024: four wavefronts share a row's K, two sets of them a block (9728 x 896 4.2; eight: 4.4);
+//   K up to 1024: as many wavefronts share a row's K as it has units of 256, in several sets (9728 x 896 in two of four 4.2, in eight 4.4;
+//     150000 x 64 in eight of one 4.8, in two of four 11.4);
 //   up to twelve units of 256 k: eight; beyond: sixteen (3584 x 18944 9.8; eight 10.8; 4608 x 3584 4.8; 5.2);
 //   32 rows a block from 4096 on, where that still makes more than half as many blocks as there are CUs (4608 x 3584 4.8, 16: 5.3;
 //     3584 x 18944 12.9, 16: 9.8), and while the scales of their rows leave room in LDS.
 template <int SRC, bool GATED>
 static hipError_t launch_row(const uint8_t* W, const uint8_t* sw, int64_t N, int64_t K, float* y, const MxRow& R) {
   const int64_t nb = K / kMxBlock, units = (nb + 7) / 8, cus = cu_count();
-  const int KW = units <= 4 ? 4 : 8;
+  const int KW = units <= 1 ? 1 : units <= 2 ? 2 : units <= 4 ? 4 : 8;
   const int64_t rows = 16 * (8 / KW);          // of a tile, gate rows if gated
   if (units <= 16 && N % 16 == 0 && N > 4 * cus * rows && rows * nb >= 16) {
     constexpr int NF = GATED ? 2 : 1;
     return (units <= KW ? launch_row_tiles<SRC, NF, GATED, 1> : launch_row_tiles<SRC, NF, GATED, 2>)(W, sw, N, K, KW, 2, y, R);
   }
-  const int waves = units <= 12 ? 8 : 16, kw = units <= 4 ? 4 : waves;
+  const int waves = units <= 12 ? 8 : 16, kw = units <= 8 ? KW : waves;
   if constexpr (GATED) return launch_rows<SRC, 2, true>(nullptr, nullptr, W, sw, 1, N, K, kw, waves, y, nullptr, nullptr, R);
   else
     return (N > 16 * cus && nb <= 1024 ? launch_rows<SRC, 2, false> : launch_rows<SRC, 1, false>)(nullptr, nullptr, W, sw, 1, N, K, kw, waves, y, nullptr,
