@@ -39,6 +39,18 @@ void* tlm_open(const char* path, int64_t max_ctx, int64_t chunk, int exact, int 
     return models::open(path, o).release();
   });
 }
+// The same with MXFP4 weights; models::open refuses them together with either flag.
+void* tlm_open_mxfp4(const char* path, int64_t max_ctx, int64_t chunk, int exact, int q4) {
+  return guarded([&]() -> void* {
+    models::options o;
+    o.max_ctx = max_ctx;
+    o.chunk = chunk;
+    o.exact = exact != 0;
+    o.q4 = q4 != 0;
+    o.mxfp4 = true;
+    return models::open(path, o).release();
+  });
+}
 // A model of the given configuration (JSON text) with seeded weights, for throughput runs. rank: of Lusadra's
 // decay inputs.
 void* tlm_random(const char* config, uint32_t seed, int64_t rank, int64_t max_ctx, int64_t chunk, int exact) {

@@ -112,13 +112,14 @@ int tlq_unicode_class(uint32_t cp) {
   return (unicode::is_letter(cp) ? 1 : 0) | (unicode::is_number(cp) ? 2 : 0) | (unicode::is_space(cp) ? 4 : 0);
 }
 
-// A model built from a GGUF file: fmt 0 = int4 groups, 1 = bf16 rows. NULL on error.
+// A model built from a GGUF file: fmt 0 = int4 groups, 1 = bf16 rows, 2 = MXFP4 blocks. NULL on error.
 void* tlq_create_from_gguf(const char* path, int fmt, int64_t max_ctx) {
   g_file_error.clear();
   auto* h = new handle();
   try {
     gguf::model g(path);
-    if (qwen::load_gguf(h->M, g, fmt == 0 ? qwen::wfmt::q4 : qwen::wfmt::bf16_row, max_ctx, &g_file_error))
+    const qwen::wfmt f = fmt == 0 ? qwen::wfmt::q4 : fmt == 2 ? qwen::wfmt::mxfp4 : qwen::wfmt::bf16_row;
+    if (qwen::load_gguf(h->M, g, f, max_ctx, &g_file_error))
       return h;
   } catch (const std::exception& e) {
     g_file_error = e.what();
@@ -162,6 +163,24 @@ int tlq_set_head_bf16(void* hv, const uint16_t* embed, const float* onorm, const
 
 int tlq_set_random_bf16(void* hv, uint32_t seed) {
   return qwen::set_random_bf16(static_cast<handle*>(hv)->M, seed) ? 0 : -1;
+}
+
+// The same blobs rounded to MXFP4 on the device.
+int tlq_set_layer_mxfp4(void* hv, int64_t li, const uint16_t* wq, const uint16_t* wk,
+                        const uint16_t* wv, const uint16_t* wo, const uint16_t* wg, const uint16_t* wu,
+                        const uint16_t* wd, const float* bq, const float* bk, const float* bv,
+                        const float* an, const float* fn) {
+  auto* h = static_cast<handle*>(hv);
+  qwen::layer_blobs_bf16 b{wq, wk, wv, wo, wg, wu, wd, bq, bk, bv, an, fn};
+  return qwen::set_layer_bf16(h->M, li, b, qwen::wfmt::mxfp4) ? 0 : -1;
+}
+
+int tlq_set_head_mxfp4(void* hv, const uint16_t* embed, const float* onorm, const uint16_t* outw) {
+  return qwen::set_head_bf16(static_cast<handle*>(hv)->M, embed, onorm, outw, qwen::wfmt::mxfp4) ? 0 : -1;
+}
+
+int tlq_set_random_mxfp4(void* hv, uint32_t seed) {
+  return qwen::set_random_mxfp4(static_cast<handle*>(hv)->M, seed) ? 0 : -1;
 }
 
 // Consume n prompt tokens in chunks, appending to the caches at their current

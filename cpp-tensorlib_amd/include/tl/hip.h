@@ -180,6 +180,20 @@ struct api {
   int (*gemm_f16w_nt_swiglu_aimage)(const void*, const void*, const void*, const void*, void*, int64_t, int64_t,
                                     int64_t) = nullptr;
   int (*attn_parts_splits)(int64_t, int64_t, int64_t, int64_t, int) = nullptr;
+  int (*quantize_mxfp4)(const void*, int, void*, void*, int64_t, int64_t) = nullptr;
+  int (*quantize_mxfp8)(const void*, void*, void*, int64_t, int64_t) = nullptr;
+  int (*dequantize_mxfp4)(const void*, const void*, void*, int, int64_t, int64_t) = nullptr;
+  int (*dequantize_mxfp8)(const void*, const void*, void*, int, int64_t, int64_t) = nullptr;
+  int (*rmsnorm_res_mxfp8)(const void*, const void*, int64_t, const void*, void*, void*, void*, int64_t, float, int64_t) = nullptr;
+  int (*gemv_mxfp4)(const void*, const void*, const void*, void*, int64_t, int64_t) = nullptr;
+  int (*gemv_mxfp4_rmsnorm)(const void*, const void*, const void*, void*, const void*, const void*, void*, int64_t, int64_t,
+                            float) = nullptr;
+  int (*gemv_mxfp4_rmsnorm_gateup)(const void*, const void*, const void*, void*, const void*, const void*, void*, int64_t, int64_t,
+                                   float) = nullptr;
+  int (*gemm_mxfp4_nt)(const void*, const void*, const void*, const void*, void*, int64_t, int64_t, int64_t) = nullptr;
+  int (*gemm_mxfp4_nt_parts)(const void*, const void*, const void*, const void*, void*, int64_t, int64_t, int64_t, int64_t,
+                             int*) = nullptr;
+  int (*gemm_mxfp4_nt_swiglu)(const void*, const void*, const void*, const void*, void*, void*, int64_t, int64_t, int64_t) = nullptr;
   int (*attn_decode_qkv_parts)(const void*, const void*, const void*, const void*, void*, void*, int64_t, int64_t,
                               int64_t, const void*, int64_t, int64_t, float, const void*, void*, int64_t,
                               int*) = nullptr;
@@ -419,6 +433,13 @@ struct context {
               bind(f.gemm_f16w_nt_parts_aimage, "tlhip_gemm_f16w_nt_parts_aimage") &&
               bind(f.gemm_f16w_nt_swiglu_aimage, "tlhip_gemm_f16w_nt_swiglu_aimage") &&
               bind(f.attn_parts_splits, "tlhip_attn_parts_splits") &&
+              bind(f.quantize_mxfp4, "tlhip_quantize_mxfp4") && bind(f.quantize_mxfp8, "tlhip_quantize_mxfp8") &&
+              bind(f.dequantize_mxfp4, "tlhip_dequantize_mxfp4") && bind(f.dequantize_mxfp8, "tlhip_dequantize_mxfp8") &&
+              bind(f.rmsnorm_res_mxfp8, "tlhip_rmsnorm_res_mxfp8") && bind(f.gemv_mxfp4, "tlhip_gemv_mxfp4") &&
+              bind(f.gemv_mxfp4_rmsnorm, "tlhip_gemv_mxfp4_rmsnorm") &&
+              bind(f.gemv_mxfp4_rmsnorm_gateup, "tlhip_gemv_mxfp4_rmsnorm_gateup") &&
+              bind(f.gemm_mxfp4_nt, "tlhip_gemm_mxfp4_nt") && bind(f.gemm_mxfp4_nt_parts, "tlhip_gemm_mxfp4_nt_parts") &&
+              bind(f.gemm_mxfp4_nt_swiglu, "tlhip_gemm_mxfp4_nt_swiglu") &&
               bind(f.attn_decode_qkv_parts, "tlhip_attn_decode_qkv_parts") &&
               bind(f.gemv_q4_attn, "tlhip_gemv_q4_attn") &&
               bind(f.gemv_bf16_row_attn, "tlhip_gemv_bf16_row_attn") &&
@@ -654,7 +675,7 @@ inline void cpu_barrier() {
 // assert that a green result was computed on the GPU (webgpu.h:197-202).
 inline std::vector<uint64_t> census() {
   auto& c = context::get();
-  std::vector<uint64_t> v(32, 0);
+  std::vector<uint64_t> v(64, 0);   // (the library fills as many as it has counters)
   if (c.ready) c.f.census(v.data(), (int)v.size());
   return v;
 }
@@ -1461,6 +1482,100 @@ inline bool gemv_bf16_row_rmsnorm_gateup(void* x, void* delta, void* norm_w, voi
   if (xout) L.writes(xout);
   L.writes(act);
   return L.sent(L.lib.gemv_bf16_row_rmsnorm_gateup(x, delta, norm_w, xout, B, act, n2, k, eps));
+}
+
+// ---- microscaled formats: MXFP4 weights (codes, scales), MXFP8 rows (codes, scales), blocks of 32 ----
+inline bool quantize_mxfp4(void* src, elem st, void* codes, void* scales, int64_t rows, int64_t K) {
+  launch L;
+  if (!L.ok || !src || !codes || !scales) return false;
+  L.reads(src);
+  L.writes(codes, scales);
+  return L.sent(L.lib.quantize_mxfp4(src, (int)st, codes, scales, rows, K));
+}
+inline bool quantize_mxfp8(void* x, void* codes, void* scales, int64_t rows, int64_t K) {
+  launch L;
+  if (!L.ok || !x || !codes || !scales) return false;
+  L.reads(x);
+  L.writes(codes, scales);
+  return L.sent(L.lib.quantize_mxfp8(x, codes, scales, rows, K));
+}
+inline bool dequantize_mxfp4(void* codes, void* scales, void* dst, elem dt, int64_t rows, int64_t K) {
+  launch L;
+  if (!L.ok || !codes || !scales || !dst) return false;
+  L.reads(codes, scales);
+  L.writes(dst);
+  return L.sent(L.lib.dequantize_mxfp4(codes, scales, dst, (int)dt, rows, K));
+}
+inline bool dequantize_mxfp8(void* codes, void* scales, void* dst, elem dt, int64_t rows, int64_t K) {
+  launch L;
+  if (!L.ok || !codes || !scales || !dst) return false;
+  L.reads(codes, scales);
+  L.writes(dst);
+  return L.sent(L.lib.dequantize_mxfp8(codes, scales, dst, (int)dt, rows, K));
+}
+// s = x + the parts (n_parts = 0: none) -> xout (optional, may be x); rmsnorm(s, w) as MXFP8 rows
+inline bool rmsnorm_res_mxfp8(void* x, void* parts, int64_t n_parts, void* w, void* xout, void* codes, void* scales, int64_t n,
+                              float eps, int64_t rows = 1) {
+  launch L;
+  if (!L.ok || !x || !w || !codes || !scales || (n_parts > 0 && !parts)) return false;
+  L.reads(x, w);
+  if (n_parts > 0) L.reads(parts);
+  if (xout) L.writes(xout);
+  L.writes(codes, scales);
+  return L.sent(L.lib.rmsnorm_res_mxfp8(x, n_parts > 0 ? parts : nullptr, n_parts, w, xout, codes, scales, n, eps, rows));
+}
+inline bool gemv_mxfp4(void* a, void* codes, void* scales, void* y, int64_t N, int64_t K) {
+  launch L;
+  if (!L.ok || (K % 32) != 0) return false;
+  L.reads(a, codes, scales);
+  L.writes(y);
+  return L.sent(L.lib.gemv_mxfp4(a, codes, scales, y, N, K));
+}
+inline bool gemv_mxfp4_rmsnorm(void* x, void* delta, void* norm_w, void* xout, void* codes, void* scales, void* y, int64_t N,
+                               int64_t K, float eps) {
+  launch L;
+  if (!L.ok || (K % 32) != 0 || (xout && (xout == x || xout == delta))) return false;
+  L.reads(x);
+  if (delta) L.reads(delta);
+  L.reads(norm_w, codes, scales);
+  if (xout) L.writes(xout);
+  L.writes(y);
+  return L.sent(L.lib.gemv_mxfp4_rmsnorm(x, delta, norm_w, xout, codes, scales, y, N, K, eps));
+}
+inline bool gemv_mxfp4_rmsnorm_gateup(void* x, void* delta, void* norm_w, void* xout, void* codes, void* scales, void* act,
+                                      int64_t N2, int64_t K, float eps) {
+  launch L;
+  if (!L.ok || (K % 32) != 0 || (N2 % 2) != 0 || (xout && (xout == x || xout == delta))) return false;
+  L.reads(x);
+  if (delta) L.reads(delta);
+  L.reads(norm_w, codes, scales);
+  if (xout) L.writes(xout);
+  L.writes(act);
+  return L.sent(L.lib.gemv_mxfp4_rmsnorm_gateup(x, delta, norm_w, xout, codes, scales, act, N2, K, eps));
+}
+// MXFP8 rows [m, k] over an MXFP4 weight [n, k]: f32 out, its K-split parts, or the gated activation as MXFP8 rows [m, ff]
+inline bool gemm_mxfp4_nt(void* acodes, void* ascales, void* codes, void* scales, void* out, int64_t m, int64_t n, int64_t k) {
+  launch L;
+  if (!L.ok || (k % 32) != 0 || m <= 0 || n <= 0) return false;
+  L.reads(acodes, ascales, codes, scales);
+  L.writes(out);
+  return L.sent(L.lib.gemm_mxfp4_nt(acodes, ascales, codes, scales, out, m, n, k));
+}
+inline bool gemm_mxfp4_nt_parts(void* acodes, void* ascales, void* codes, void* scales, void* parts, int64_t parts_bytes, int64_t m,
+                                int64_t n, int64_t k, int* n_parts) {
+  launch L;
+  if (!L.ok || (k % 32) != 0 || m <= 0 || n <= 0 || !n_parts) return false;
+  L.reads(acodes, ascales, codes, scales);
+  L.writes(parts);
+  return L.sent(L.lib.gemm_mxfp4_nt_parts(acodes, ascales, codes, scales, parts, parts_bytes, m, n, k, n_parts));
+}
+inline bool gemm_mxfp4_nt_swiglu(void* acodes, void* ascales, void* codes, void* scales, void* act_codes, void* act_scales, int64_t m,
+                                 int64_t ff, int64_t k) {
+  launch L;
+  if (!L.ok || (k % 32) != 0 || (ff % 32) != 0 || m <= 0 || ff <= 0) return false;
+  L.reads(acodes, ascales, codes, scales);
+  L.writes(act_codes, act_scales);
+  return L.sent(L.lib.gemm_mxfp4_nt_swiglu(acodes, ascales, codes, scales, act_codes, act_scales, m, ff, k));
 }
 
 // ---- events on the library's stream: GPU time between two points of the launch sequence ------

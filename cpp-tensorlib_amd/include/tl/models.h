@@ -27,6 +27,7 @@ struct options {
   int64_t chunk = 512;         // longest prompt chunk
   bool exact = false;          // prompt products exact in f32, not in two rounded terms per operand
   bool q4 = false;             // int4 weights (models loaded from GGUF)
+  bool mxfp4 = false;          // MXFP4 weights, MXFP8 rows in prompt chunks (models loaded from GGUF)
 };
 
 // Models that offer what measuring and checking layer by layer needs: launch forms, the residual stream
@@ -171,7 +172,8 @@ inline std::unique_ptr<any> open_gguf(const std::string& path, const options& o)
   auto p = std::make_unique<of<qwen::model>>("qwen2", o.chunk);
   p->m.prompt_f16 = !o.exact;
   std::string why;
-  if (!qwen::load_gguf(p->m, g, o.q4 ? qwen::wfmt::q4 : qwen::wfmt::bf16_row, o.max_ctx, &why)) throw std::runtime_error(why);
+  const qwen::wfmt fmt = o.mxfp4 ? qwen::wfmt::mxfp4 : o.q4 ? qwen::wfmt::q4 : qwen::wfmt::bf16_row;
+  if (!qwen::load_gguf(p->m, g, fmt, o.max_ctx, &why)) throw std::runtime_error(why);
   return p;
 }
 
@@ -186,8 +188,10 @@ inline json::value read_config(const std::string& dir) {
 // Throws std::runtime_error with the reason.
 inline std::unique_ptr<any> open(const std::string& path, const options& o) {
   struct stat st;
+  if (o.mxfp4 && (o.q4 || o.exact)) throw std::runtime_error(path + ": MXFP4 weights exclude int4 ones and exact prompt products");
   if (::stat(path.c_str(), &st) != 0) throw std::runtime_error(path + ": not found");
   if (!S_ISDIR(st.st_mode)) return open_gguf(path, o);
+  if (o.mxfp4) throw std::runtime_error(path + ": MXFP4 weights are for models loaded from GGUF");
   const json::value cfg = read_config(path);
   return folder_entry(cfg, path).open(cfg, path, o);
 }

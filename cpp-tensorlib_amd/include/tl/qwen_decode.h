@@ -22,7 +22,8 @@
 // qm:357-395): the same layer wiring with every GEMV replaced by the MFMA GEMM
 // over [T, hidden] activations, split_heads/rope/kv_fill/attn_prefill/merge_heads
 // around the cache, and multi-row norms. Like the reference's, it needs bf16
-// row-major weights.
+// row-major weights; int4 and MXFP4 weights have chunks here as well, the latter over
+// MXFP8 activations (prefill_layers_mx).
 
 #include <algorithm>
 #include <cmath>
@@ -229,13 +230,29 @@ inline bool set_layer_q4(model& M, int64_t li, const layer_blobs& b) {
 
 // The same layer from bf16 blobs in the reference's logical [K,N] layout
 // (array.h:639-658): transposed on the host to [N,K] rows, the layout the decode
-// GEMV and the prefill GEMM share (qm:118-146 does this transpose at load).
+// GEMV and the prefill GEMM share (qm:118-146 does this transpose at load), or rounded from there to MXFP4.
 struct layer_blobs_bf16 {
   const uint16_t *wq, *wk, *wv, *wo, *wg, *wu, *wd;
   const float *bq, *bk, *bv, *an, *fn;
 };
 
-inline bool set_layer_bf16(model& M, int64_t li, const layer_blobs_bf16& b) {
+namespace detail {
+// bf16 rows of the host as a weight of the device in `fmt`: bf16_row or mxfp4 (rounded on the device)
+inline linear rows_as(const uint16_t* rows, int64_t N, int64_t K, wfmt fmt) {
+  if (fmt != wfmt::mxfp4) return linear{dev_from_host(rows, N * K * 2), N, K, wfmt::bf16_row};
+  linear L{hip::alloc_device(mxfp4_bytes(N, K)), N, K, wfmt::mxfp4};
+  void* stage = hip::alloc_device(N * K * 2);
+  const bool ok = L.w && stage && hip::upload_raw(stage, rows, N * K * 2) &&
+                  hip::quantize_mxfp4(stage, hip::elem::bf16, L.w, L.block_scales(), N, K);
+  hip::flush();   // the staging buffer goes
+  if (stage) hip::release(stage, 0, nullptr);
+  if (!ok && L.w) hip::release(L.w, 0, nullptr);
+  if (!ok) L.w = nullptr;
+  return L;
+}
+}  // namespace detail
+
+inline bool set_layer_bf16(model& M, int64_t li, const layer_blobs_bf16& b, wfmt fmt = wfmt::bf16_row) {
   const dims& d = M.d;
   layer& L = M.layers[(size_t)li];
   const int64_t E = d.hidden;
@@ -249,7 +266,7 @@ inline bool set_layer_bf16(model& M, int64_t li, const layer_blobs_bf16& b) {
       detail::transpose_kn(parts[i], rows.data() + n0 * K, K, Ns[i]);
       n0 += Ns[i];
     }
-    return linear{detail::dev_from_host(rows.data(), N * K * 2), N, K, wfmt::bf16_row};
+    return detail::rows_as(rows.data(), N, K, fmt);
   };
   L.wqkv = put({b.wq, b.wk, b.wv}, {d.q_dim(), d.kv_dim(), d.kv_dim()}, E);
   L.wgu = put({b.wg, b.wu}, {d.ff, d.ff}, E);
@@ -283,14 +300,13 @@ inline bool set_embed(model& M, const void* rows, bool f16) {
 }
 
 inline bool set_head_bf16(model& M, const uint16_t* embed_bf16, const float* onorm,
-                          const uint16_t* outw_kn) {
+                          const uint16_t* outw_kn, wfmt fmt = wfmt::bf16_row) {
   const dims& d = M.d;
   if (!set_embed(M, embed_bf16, false)) return false;
   M.onorm = detail::dev_from_host(onorm, d.hidden * 4);
   std::vector<uint16_t> rows((size_t)(d.vocab * d.hidden));
   detail::transpose_kn(outw_kn, rows.data(), d.hidden, d.vocab);
-  M.lm_head = linear{detail::dev_from_host(rows.data(), d.vocab * d.hidden * 2), d.vocab, d.hidden,
-                     wfmt::bf16_row};
+  M.lm_head = detail::rows_as(rows.data(), d.vocab, d.hidden, fmt);
   M.ready = M.onorm && M.lm_head.w;
   return M.ready;
 }
@@ -328,6 +344,11 @@ inline bool set_random(model& M, uint32_t seed, wfmt fmt) {
   std::vector<uint32_t> bfw((size_t)blk / 4);
   for (auto& v : bfw) v = (next() & 0x807f807fu) | 0x3c003c00u;
   void* db = fmt == wfmt::bf16_row ? detail::dev_from_host(bfw.data(), blk) : nullptr;
+  // mxfp4: the nibbles are the codes; block scales 2^-9 or 2^-8, so |w| ~ 0.01 as well
+  if (fmt == wfmt::mxfp4) {
+    for (auto& v : bfw) v = (v & 0x01010101u) + 0x76767676u;
+    db = detail::dev_from_host(bfw.data(), blk);
+  }
   auto make = [&](int64_t N, int64_t K) {
     if (fmt == wfmt::bf16_row) {
       linear L{hip::alloc_device(N * K * 2), N, K, wfmt::bf16_row};
@@ -336,13 +357,14 @@ inline bool set_random(model& M, uint32_t seed, wfmt fmt) {
         ok &= hip::copy_d2d(static_cast<char*>(L.w) + o, db, std::min(blk, N * K * 2 - o));
       return L;
     }
-    linear L{hip::alloc_device(q4_bytes(N, K)), N, K, wfmt::q4};
-    if (!L.w) { ok = false; return L; }
-    const int64_t pb = N * K / 2, sb = N * (K / kQ4Group) * 4;
+    linear L{nullptr, N, K, fmt};
+    L.w = hip::alloc_device(L.bytes());
+    if (!L.w || (fmt == wfmt::mxfp4 && !db)) { ok = false; return L; }
+    const int64_t pb = N * K / 2, sb = L.bytes() - pb;
     for (int64_t o = 0; o < pb; o += blk)
       ok &= hip::copy_d2d(static_cast<char*>(L.w) + o, dn, std::min(blk, pb - o));
     for (int64_t o = 0; o < sb; o += blk)
-      ok &= hip::copy_d2d(static_cast<char*>(L.w) + pb + o, ds, std::min(blk, sb - o));
+      ok &= hip::copy_d2d(static_cast<char*>(L.w) + pb + o, fmt == wfmt::mxfp4 ? db : ds, std::min(blk, sb - o));
     return L;
   };
   auto hvec = [&](int64_t n, float mean, float std_) {
@@ -371,6 +393,7 @@ inline bool set_random(model& M, uint32_t seed, wfmt fmt) {
 }
 inline bool set_random_q4(model& M, uint32_t seed) { return set_random(M, seed, wfmt::q4); }
 inline bool set_random_bf16(model& M, uint32_t seed) { return set_random(M, seed, wfmt::bf16_row); }
+inline bool set_random_mxfp4(model& M, uint32_t seed) { return set_random(M, seed, wfmt::mxfp4); }
 
 // Fill every layer's cache rows [0, upto) with seeded N(0,1)-like values so a
 // decode step at a deep position reads a realistic cache.
@@ -403,7 +426,8 @@ inline bool fill_cache_random(model& M, int64_t upto, uint32_t seed) {
 // narrows to bf16 / quantises to int4 and uploads the result. Here the mapped file bytes go
 // to the device as they are, through one staging buffer, and tlhip_convert /
 // tlhip_quantize_q4 write the decode formats straight into the fused weight buffers:
-// the same values bit for bit, with the element loops on the GPU.
+// the same values bit for bit, with the element loops on the GPU. tlhip_quantize_mxfp4
+// does the same into MXFP4, which the reference has not.
 namespace detail {
 
 inline bool why_(std::string* why, const std::string& msg) {
@@ -451,6 +475,8 @@ struct converter {
       if (dst.fmt == wfmt::q4)
         ok = hip::quantize_q4(stage, e, w + row * in / 2,
                               w + dst.N * in / 2 + row * (in / kQ4Group) * 4, n, in);
+      else if (dst.fmt == wfmt::mxfp4)
+        ok = hip::quantize_mxfp4(stage, e, w + row * in / 2, static_cast<char*>(dst.block_scales()) + row * (in / 32), n, in);
       else
         ok = hip::convert(stage, e, w + row * in * 2, hip::elem::bf16, n * in);
       if (!ok) return false;
@@ -519,7 +545,7 @@ inline bool dims_from_gguf(const gguf::model& g, int64_t max_ctx, dims& d, std::
   return true;
 }
 
-// Builds the model from a mapped file: linear layers into `fmt` (int4 groups or bf16 rows),
+// Builds the model from a mapped file: linear layers into `fmt` (int4 groups, bf16 rows or MXFP4),
 // fused [q|k|v] and [gate|up] by stacking row blocks; norms and biases f32; the embedding
 // stays in the file's f16 (bf16 accepted) and is gathered per token. output.weight may be
 // absent (tied to token_embd.weight).
@@ -628,7 +654,8 @@ inline bool run_layers(model& M, void* x0, int64_t pos, void* logits_out = nullp
     if (!M.rope_tab) M.rope_tab = hip::alloc_device(d.head_dim * 4);
     ok &= M.rope_tab && hip::rope_table(M.rope_tab, d.head_dim, pos, d_pos, d.rope_base);
     // the attention's splits merged by the o-projection: decided once per step from the launch plan
-    const bool merge = M.fused_attn && M.merge_in_oproj && M.attn_partials &&
+    // (an MXFP4 o-projection takes the merged row only)
+    const bool merge = M.fused_attn && M.merge_in_oproj && M.attn_partials && M.layers[0].wo.fmt != wfmt::mxfp4 &&
                        hip::attn_parts_splits(d.n_q_heads, d.n_kv_heads, d_pos ? M.layers[0].cache.max_ctx : pos + 1,
                                               d.head_dim, M.layers[0].cache.kv_bf16) > 0;
     size_t marks = 0;
@@ -669,7 +696,7 @@ inline bool run_layers(model& M, void* x0, int64_t pos, void* logits_out = nullp
       mark();
       ok &= merge ? gemv_attn(L.wo, M.attn_partials, n_parts, d.n_q_heads, d.head_dim, S.hb) : gemv(L.wo, S.ab, S.hb);
       mark();
-      if (M.gateup_epilogue) {
+      if (M.gateup_epilogue || L.wd.fmt == wfmt::mxfp4) {   // MXFP4 has the gate as an epilogue only
         ok &= gemv_rmsnorm_gateup(L.wgu, S.res[0], S.hb, L.fn, S.res[1], S.mb, d.eps);
         mark();
         ok &= gemv(L.wd, S.mb, S.mdb);
@@ -779,12 +806,46 @@ inline bool prefill_reserve(model& M, int64_t T) {
   return ok;
 }
 
+// Chunks over MXFP4 weights (no reference counterpart): every product reads MXFP8 rows, which its producer writes - the norms,
+// the gate's epilogue, and one rounding of the attention's rows; the residual, the caches and the attention stay f32. The rows lie
+// in scratch that these chunks have no other use for. Decode steps take f32 rows, so a token's logits differ between the
+// two by the rounding of the chunk's activations.
+inline bool prefill_layers_mx(model& M, int64_t T) {
+  const dims& d = M.d;
+  prefill_scratch& P = M.ps;
+  const float scale = 1.0f / std::sqrt((float)d.head_dim);
+  const int64_t E = d.hidden, pos0 = M.layers[0].cache.pos;
+  const mx_rows h(P.h2, T, E), at(P.ah, T, d.q_dim()), act(P.mb, T, d.ff);
+  void* x = P.emb;
+  int np = 0;
+  bool ok = hip::rope_table_range(P.rope, d.head_dim, pos0, T, d.rope_base) &&
+            hip::rmsnorm_res_mxfp8(x, nullptr, 0, M.layers[0].an, nullptr, h.codes, h.scales, E, d.eps, T);
+  for (int64_t l = 0; l < d.n_layers && ok; l++) {
+    layer& L = M.layers[(size_t)l];
+    void* ro = P.res[l & 1];
+    ok = gemm_parts(L.wqkv, h, P.parts, P.parts_bytes, T, &np);
+    L.cache.pos = pos0;
+    ok = ok && L.cache.prefill_qkv(P.parts, L.bq, L.bk, L.bv, P.rope, P.qkvh, P.at, T, d.n_q_heads, scale, np) &&
+         hip::quantize_mxfp8(P.at, at.codes, at.scales, T, d.q_dim()) &&
+         gemm_parts(L.wo, at, P.parts, P.parts_bytes, T, &np) &&
+         hip::rmsnorm_res_mxfp8(x, P.parts, np, L.fn, ro, h.codes, h.scales, E, d.eps, T) &&
+         gemm_swiglu(L.wgu, h, act, T) && gemm_parts(L.wd, act, P.parts, P.parts_bytes, T, &np);
+    if (l + 1 < d.n_layers)
+      ok = ok && hip::rmsnorm_res_mxfp8(ro, P.parts, np, M.layers[(size_t)l + 1].an, ro, h.codes, h.scales, E, d.eps, T);
+    else   // the head's rows are f32
+      ok = ok && hip::rmsnorm_res_parts(ro, P.parts, np, M.onorm, ro, P.h, E, d.eps, T);
+    x = ro;
+  }
+  return ok;
+}
+
 // All layers over the T rows staged in ps.emb, appended to the caches at their
 // current position (qm:357-395). Leaves the final norm of every row in ps.h.
 inline bool prefill_layers(model& M, int64_t T) {
   const dims& d = M.d;
   prefill_scratch& P = M.ps;
   if (T <= 0 || T > P.T) return false;
+  if (M.layers[0].wqkv.fmt == wfmt::mxfp4) return prefill_layers_mx(M, T);
   for (const layer& L : M.layers)   // the MFMA GEMM reads bf16 rows or int4, not [K,N] bf16
     if (L.wqkv.fmt != wfmt::bf16_row && L.wqkv.fmt != wfmt::q4) return false;
   const float scale = 1.0f / std::sqrt((float)d.head_dim);

@@ -20,6 +20,7 @@ def _load():
         sig = {
             "tlm_error": (C.c_char_p, []),
             "tlm_open": (P, [C.c_char_p, i64, i64, cint, cint]),
+            "tlm_open_mxfp4": (P, [C.c_char_p, i64, i64, cint, cint]),
             "tlm_random": (P, [C.c_char_p, u32, i64, i64, i64, cint]),
             "tlm_close": (None, [P]),
             "tlm_architecture": (C.c_char_p, [P]),
@@ -60,10 +61,11 @@ class Model:
         self.vocab, self.capacity = int(L.tlm_vocab(h)), int(L.tlm_capacity(h))
 
     @classmethod
-    def open(cls, path, max_ctx=4096, chunk=512, exact=False, q4=False):
-        """exact: prompt products exact in f32 instead of in two rounded terms per operand."""
+    def open(cls, path, max_ctx=4096, chunk=512, exact=False, q4=False, mxfp4=False):
+        """exact: prompt products exact in f32 instead of in two rounded terms per operand; q4, mxfp4: the weights of a
+        GGUF file in int4 groups or in MXFP4 blocks (prompt chunks then round their activations to MXFP8)."""
         L = _load()
-        return cls(L, L.tlm_open(os.fsencode(path), max_ctx, chunk, int(exact), int(q4)))
+        return cls(L, (L.tlm_open_mxfp4 if mxfp4 else L.tlm_open)(os.fsencode(path), max_ctx, chunk, int(exact), int(q4)))
 
     @classmethod
     def random(cls, config, seed=1, rank=16, max_ctx=4096, chunk=512, exact=False):

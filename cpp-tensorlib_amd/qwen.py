@@ -46,6 +46,9 @@ def _load():
             "tlq_set_layer_bf16": (cint, [P, i64] + [P] * 12),
             "tlq_set_head_bf16": (cint, [P, P, P, P]),
             "tlq_set_random_bf16": (cint, [P, u32]),
+            "tlq_set_layer_mxfp4": (cint, [P, i64] + [P] * 12),
+            "tlq_set_head_mxfp4": (cint, [P, P, P, P]),
+            "tlq_set_random_mxfp4": (cint, [P, u32]),
             "tlq_prefill": (cint, [P, P, i64, i64, P]),
             "tlq_stage_chunk": (cint, [P, P, i64]),
             "tlq_prefill_layers": (cint, [P, i64, i64]),
@@ -188,12 +191,12 @@ class QwenGPU:
     def from_blobs(cls, om, fmt="q4"):
         """Build from a weight source: any object with `.d` (the dims) and
         `.weight(layer, name)` returning the stored bytes of wq/wk/wv/wo/wg/wu/wd (q4
-        buffers, or bf16 in the logical [K,N] layout when fmt == "bf16"), bq/bk/bv/an/fn
-        (f32) and, for layer -1, embed (bf16), onorm, outw."""
+        buffers, or bf16 in the logical [K,N] layout when fmt == "bf16", or "mxfp4", which rounds
+        those to MXFP4 on the device), bq/bk/bv/an/fn (f32) and, for layer -1, embed (bf16), onorm, outw."""
         d = om.d
         g = cls(dict((f, getattr(d, f)) for f, _ in Dims._fields_))
-        set_layer = g.L.tlq_set_layer_q4 if fmt == "q4" else g.L.tlq_set_layer_bf16
-        set_head = g.L.tlq_set_head_q4 if fmt == "q4" else g.L.tlq_set_head_bf16
+        set_layer = g.L.tlq_set_layer_q4 if fmt == "q4" else g.L.tlq_set_layer_mxfp4 if fmt == "mxfp4" else g.L.tlq_set_layer_bf16
+        set_head = g.L.tlq_set_head_q4 if fmt == "q4" else g.L.tlq_set_head_mxfp4 if fmt == "mxfp4" else g.L.tlq_set_head_bf16
         for li in range(d.n_layers):
             w = [np.ascontiguousarray(om.weight(li, n)) for n in ("wq", "wk", "wv", "wo", "wg", "wu", "wd")]
             v = [np.ascontiguousarray(om.weight(li, n)) for n in ("bq", "bk", "bv", "an", "fn")]
@@ -209,12 +212,12 @@ class QwenGPU:
     @classmethod
     def from_gguf(cls, path, fmt="q4", max_ctx=4096):
         """Build from a GGUF file: f16 / f32 / bf16 tensors are uploaded as stored and converted to
-        int4 groups (fmt "q4") or bf16 rows (fmt "bf16") on the device."""
+        int4 groups (fmt "q4"), bf16 rows (fmt "bf16") or MXFP4 blocks (fmt "mxfp4") on the device."""
         g = cls.__new__(cls)
         g.L = _load()
         if not g.L.tlq_available():
             raise RuntimeError("tl::hip backend unavailable: %s" % g.L.tlq_unavailable_reason().decode())
-        g.h = g.L.tlq_create_from_gguf(os.fsencode(path), 0 if fmt == "q4" else 1, max_ctx)
+        g.h = g.L.tlq_create_from_gguf(os.fsencode(path), 0 if fmt == "q4" else 2 if fmt == "mxfp4" else 1, max_ctx)
         if not g.h:
             raise RuntimeError("load_gguf failed: %s" % g.L.tlq_file_error().decode())
         g.d = Dims()
@@ -223,7 +226,7 @@ class QwenGPU:
         return g
 
     def set_random(self, seed=1, fmt="q4"):
-        fn = self.L.tlq_set_random_q4 if fmt == "q4" else self.L.tlq_set_random_bf16
+        fn = self.L.tlq_set_random_q4 if fmt == "q4" else self.L.tlq_set_random_mxfp4 if fmt == "mxfp4" else self.L.tlq_set_random_bf16
         if fn(self.h, seed) != 0:
             raise RuntimeError("set_random failed")
 
