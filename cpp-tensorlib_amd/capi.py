@@ -153,6 +153,7 @@ SIGNATURES = {
     "tlhip_dequantize_mxfp8": (cint, [P, P, P, cint, i64, i64]),
     "tlhip_rmsnorm_res_mxfp8": (cint, [P, P, i64, P, P, P, P, i64, f32, i64]),
     "tlhip_gemv_mxfp4": (cint, [P, P, P, P, i64, i64]),
+    "tlhip_gemv_mxfp4_attn": (cint, [P, i64, i64, i64, P, P, P, i64, i64]),
     "tlhip_gemv_mxfp4_rmsnorm": (cint, [P, P, P, P, P, P, P, i64, i64, f32]),
     "tlhip_gemv_mxfp4_rmsnorm_gateup": (cint, [P, P, P, P, P, P, P, i64, i64, f32]),
     "tlhip_gemm_mxfp4_nt": (cint, [P, P, P, P, P, i64, i64, i64]),
@@ -592,6 +593,9 @@ class TlHip:
 
     def gemv_mxfp4(self, a, codes, scales, y, N, K):
         self._chk(self.c.tlhip_gemv_mxfp4(a.ptr, codes.ptr, scales.ptr, y.ptr, N, K))
+
+    def gemv_mxfp4_attn(self, parts, n_parts, heads, D, codes, scales, y, N, K):
+        self._chk(self.c.tlhip_gemv_mxfp4_attn(parts.ptr, n_parts, heads, D, codes.ptr, scales.ptr, y.ptr, N, K))
 
     def gemv_mxfp4_rmsnorm(self, x, delta, norm_w, xout, codes, scales, y, N, K, eps):
         self._chk(self.c.tlhip_gemv_mxfp4_rmsnorm(x.ptr, delta.ptr if delta is not None else None, norm_w.ptr,

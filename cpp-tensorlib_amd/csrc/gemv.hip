@@ -953,6 +953,17 @@ static int check_gemv_args(const void* a, const void* B, const void* y, int64_t 
 
 using namespace tlhip;
 
+int tlhip::check_attn_merge(const void* parts, int64_t n_parts, int64_t heads, int64_t D, int64_t K, const char* who) {
+  if (!parts || !aligned16(parts)) return fail(TLHIP_EINVAL, "%s: partials pointer null or not 16-byte aligned", who);
+  if (heads <= 0 || heads > 4096 || (D != 64 && D != 128) || heads * D != K)
+    return fail(TLHIP_EINVAL, "%s: K must be heads x head_dim, head_dim 64 or 128", who);
+  // as many splits as the merge kernel has groups, which it sums one after the other
+  const int64_t most = D == 64 ? kMergeMax : kMergeMax / 2;
+  if (n_parts < 1 || n_parts > most) return fail(TLHIP_EUNSUPPORTED, "%s: 1 to %d split partials", who, (int)most);
+  if (((2 * heads * n_parts) % 4) != 0) return fail(TLHIP_EUNSUPPORTED, "%s: heads x splits must be even", who);
+  return 0;
+}
+
 extern "C" {
 
 int tlhip_gemv_q4(const void* a, const void* qw, const void* scales, void* y, int64_t N,
@@ -985,17 +996,6 @@ int tlhip_gemv_bf16_row(const void* a, const void* W, void* y, int64_t n, int64_
     return fail(TLHIP_EUNSUPPORTED, "tlhip_gemv_bf16_row: K too large for the LDS-staged kernel");
   return launch_rows<FmtBf16>(static_cast<const float*>(a), W, nullptr, static_cast<float*>(y), n, k,
                               TLHIP_C_GEMV_BF16_ROW);
-}
-
-static int check_attn_merge(const void* parts, int64_t n_parts, int64_t heads, int64_t D, int64_t K, const char* who) {
-  if (!parts || !aligned16(parts)) return fail(TLHIP_EINVAL, "%s: partials pointer null or not 16-byte aligned", who);
-  if (heads <= 0 || heads > 4096 || (D != 64 && D != 128) || heads * D != K)
-    return fail(TLHIP_EINVAL, "%s: K must be heads x head_dim, head_dim 64 or 128", who);
-  // as many splits as the merge kernel has groups, which it sums one after the other
-  const int64_t most = D == 64 ? kMergeMax : kMergeMax / 2;
-  if (n_parts < 1 || n_parts > most) return fail(TLHIP_EUNSUPPORTED, "%s: 1 to %d split partials", who, (int)most);
-  if (((2 * heads * n_parts) % 4) != 0) return fail(TLHIP_EUNSUPPORTED, "%s: heads x splits must be even", who);
-  return 0;
 }
 
 int tlhip_gemv_q4_attn(const void* parts, int64_t n_parts, int64_t heads, int64_t head_dim, const void* qw,

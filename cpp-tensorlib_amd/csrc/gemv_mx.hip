@@ -22,20 +22,73 @@ namespace tlhip {
 // The scales of a block's rows are one run of bytes: copied into LDS whole (a byte loaded by each lane was a request for 16 lines: 70 us
 // instead of 60 over 152064 x 3584).
 typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(1)));
-__device__ __forceinline__ void put_scales(char* to, const uint8_t* from, int bytes, int64_t limit, int tid, int threads) {
+// (two runs `apart` bytes from each other: both asked for before either is waited for, 4608 x 3584 with the gate 10.2 us one by one)
+__host__ __device__ constexpr int whole_16(int bytes) { return (bytes + 15) & ~15; }
+template <int RUNS>
+__device__ __forceinline__ void put_scales(char* to, const uint8_t* from, int64_t apart, int bytes, int64_t limit, int tid, int threads) {
   for (int i = 16 * tid; i < bytes; i += 16 * threads) {
-    if (i + 16 <= limit)
-      *reinterpret_cast<frag16*>(to + i) = *reinterpret_cast<const any16*>(from + i);
-    else
-      for (int k = 0; k < 16 && i + k < limit; k++) to[i + k] = (char)from[i + k];
+    if (i + 16 <= limit) {
+      any16 v[RUNS];
+#pragma unroll
+      for (int k = 0; k < RUNS; k++) v[k] = *reinterpret_cast<const any16*>(from + k * apart + i);
+#pragma unroll
+      for (int k = 0; k < RUNS; k++) *reinterpret_cast<frag16*>(to + k * whole_16(bytes) + i) = v[k];
+    } else {
+      for (int k = 0; k < RUNS; k++)
+        for (int j = 0; j < 16 && i + j < limit; j++) to[k * whole_16(bytes) + i + j] = (char)from[k * apart + i + j];
+    }
   }
 }
-enum { kCodes = 0, kFloat = 1, kNormed = 2 };
+enum { kCodes = 0, kFloat = 1, kNormed = 2, kMerged = 3 };
 struct MxRow {               // the f32 row: x (+ delta), its norm weights, and where x + delta goes
   const float *x, *delta, *norm_w;
   float* xout;
   float eps;
+  int splits, heads, dim;    // kMerged: x is the attention's partials
 };
+// Numbers k .. k + 3 of the attention's row from its splits (maxima [heads][S], sums [heads][S], accumulators [heads][S][dim], as
+// tlhip_attn_decode_qkv_parts leaves them): sum_s e^(m_s - M) acc_s / sum_s e^(m_s - M) l_s in the order of tlhip_gemv_q4_attn's merge.
+// The 16 lanes of a row have numbers of one head (dim is 64 or 128) and the weight of one split each.
+struct MergeIn {
+  static constexpr int kFirst = 8;             // splits asked for ahead of the weights
+  float m, l;
+  float4 a[kFirst];
+  const float4* acc;
+};
+__device__ __forceinline__ MergeIn ask_merge(const MxRow& R, int k, int lane) {
+  const int S = R.splits, h = k / R.dim, d = k - h * R.dim, s = min(lane & 15, S - 1), hs = R.heads * S;
+  MergeIn q;
+  q.m = R.x[h * S + s];
+  q.l = R.x[hs + h * S + s];
+  q.acc = reinterpret_cast<const float4*>(R.x + 2 * hs + (int64_t)h * S * R.dim + d);
+#pragma unroll
+  for (int i = 0; i < MergeIn::kFirst; i++) q.a[i] = q.acc[min(i, S - 1) * (R.dim / 4)];
+  return q;
+}
+__device__ __forceinline__ float4 merged(const MxRow& R, const MergeIn& q, int lane) {
+  const int S = R.splits;
+  const float m = q.m, l = q.l;
+  float M = fmaxf(m, dpp_read<0x128>(m));      // row_ror:8, 4, 2, 1
+  M = fmaxf(M, dpp_read<0x124>(M));
+  M = fmaxf(M, dpp_read<0x122>(M));
+  M = fmaxf(M, dpp_read<0x121>(M));
+  const float w = (lane & 15) < S ? __expf(m - M) : 0.f;
+  float L = mul_rn(l, w);
+  L = add_rn(L, dpp_read<0x128>(L));
+  L += dpp_read<0x124>(L);
+  L += dpp_read<0x122>(L);
+  L += dpp_read<0x121>(L);
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  const auto add = [&](int i, const float4 p) {
+    const float f = __shfl(w, (lane & 48) + i);
+    v = make_float4(add_rn(v.x, mul_rn(f, p.x)), add_rn(v.y, mul_rn(f, p.y)), add_rn(v.z, mul_rn(f, p.z)), add_rn(v.w, mul_rn(f, p.w)));
+  };
+#pragma unroll
+  for (int i = 0; i < MergeIn::kFirst; i++)
+    if (i < S) add(i, q.a[i]);
+  for (int i = MergeIn::kFirst; i < S; i++) add(i, q.acc[i * (R.dim / 4)]);
+  return make_float4(v.x / L, v.y / L, v.z / L, v.w / L);
+}
 constexpr int kDigits = 12, kUnitLds = 2 * kDigits * 128 + 16;      // digits of a unit, its eight blocks' exponents
 
 // Numbers 4 lane .. 4 lane + 3 of a unit into LDS: a step's digits [kDigits][128] bytes, then the next one's, then the exponents
@@ -88,6 +141,16 @@ __device__ __forceinline__ float join_digits(const v4f& c, int r) {
   return mine * 256.0f;
 }
 
+// Row r of tile f of a wavefront: a feature, counted from the wavefront's first. With a gate half the tiles are of gate rows,
+// the others of the up rows of the same features; one tile alone has eight of each, gate rows first.
+struct TileRow { int n; bool up; };
+template <int NF, bool GATED>
+__device__ __forceinline__ TileRow tile_row(int f, int r) {
+  if constexpr (!GATED) return {16 * f + r, false};
+  else if constexpr (NF == 1) return {r & 7, r >= 8};
+  else return {16 * (f % (NF / 2)) + r, f >= NF / 2};
+}
+
 template <int SRC, int NF, bool GATED>
 __global__ __launch_bounds__(SRC == kCodes ? 512 : 1024, 2) void mx_rows_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ sa,
                                                          const uint8_t* __restrict__ W, const uint8_t* __restrict__ sw, int M, int N, int nb, int KW,
@@ -103,10 +166,9 @@ __global__ __launch_bounds__(SRC == kCodes ? 512 : 1024, 2) void mx_rows_kernel(
   int wscale[NF];                                              // in the block's run of scales: gate rows first
 #pragma unroll
   for (int f = 0; f < NF; f++) {
-    const int n = min(n0 + 16 * (GATED ? f % (NF / 2) : f) + r, N - 1);
-    const bool up = GATED && f >= NF / 2;
-    wrow[f] = W + ((up ? (int64_t)N : 0) + n) * nb * 16;
-    wscale[f] = (fw * kTile + 16 * (GATED ? f % (NF / 2) : f) + r + (up ? FW * kTile : 0)) * nb;
+    const TileRow t = tile_row<NF, GATED>(f, r);
+    wrow[f] = W + ((t.up ? (int64_t)N : 0) + min(n0 + t.n, N - 1)) * nb * 16;
+    wscale[f] = (fw * kTile + t.n) * nb + (t.up ? whole_16(FW * kTile * nb) : 0);
   }
   const uint8_t *arow = A + (int64_t)min(r, M - 1) * nb * 32, *ascale = sa + (int64_t)min(r, M - 1) * nb;
   struct Unit {
@@ -117,7 +179,9 @@ __global__ __launch_bounds__(SRC == kCodes ? 512 : 1024, 2) void mx_rows_kernel(
   };
   // Past the end of a row: its last block or numbers again, under scales of 2^-127 on both sides (digits: as zeros)
   const auto ask = [&](Unit& q, int u) {
-    if constexpr (SRC != kCodes) {
+    MergeIn in;
+    if constexpr (SRC == kMerged) in = ask_merge(R, min(256 * u + 4 * lane, K - 4), lane);
+    if constexpr (SRC == kFloat || SRC == kNormed) {
       const int k = min(256 * u + 4 * lane, K - 4);
       q.x = *reinterpret_cast<const float4*>(R.x + k);
       if constexpr (SRC == kNormed) {
@@ -140,6 +204,7 @@ __global__ __launch_bounds__(SRC == kCodes ? 512 : 1024, 2) void mx_rows_kernel(
         q.as[h] = b < nb ? ascale[at] : 0;
       }
     }
+    if constexpr (SRC == kMerged) q.x = merged(R, in, lane);     // (the weights are on their way)
   };
   v4f c[NF];
 #pragma unroll
@@ -194,8 +259,7 @@ __global__ __launch_bounds__(SRC == kCodes ? 512 : 1024, 2) void mx_rows_kernel(
     const int rows = FW * kTile, bytes = rows * nb, first = (int)blockIdx.x * rows;
     char* const to = lds + (reinterpret_cast<const char*>(run) - lds);
     const int64_t left = (int64_t)(N - first) * nb;
-    put_scales(to, sw + (int64_t)first * nb, bytes, left, tid, 64 * waves);
-    if (GATED) put_scales(to + bytes, sw + ((int64_t)N + first) * nb, bytes, left, tid, 64 * waves);
+    put_scales<GATED ? 2 : 1>(to, sw + (int64_t)first * nb, (int64_t)N * nb, bytes, left, tid, 64 * waves);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -243,12 +307,17 @@ __global__ __launch_bounds__(SRC == kCodes ? 512 : 1024, 2) void mx_rows_kernel(
     float out[NF];
 #pragma unroll
     for (int f = 0; f < NF; f++)
-      if (my_tile(f)) out[f] = join_digits(c[f], r) * inv;
+      if (GATED || my_tile(f)) out[f] = join_digits(c[f], r) * inv;
     const int n = n0 + 4 * g + r;
     if constexpr (GATED) {
+      if constexpr (NF == 1) {
+        const float up = __shfl(out[0], (lane + 32) & 63);
+        if (kw == 0 && r < 4 && g < 2 && n < N) C[n] = gated(out[0], up);
+      } else {
 #pragma unroll
-      for (int f = 0; f < NF / 2; f++)
-        if (kw == 0 && r < 4 && n + 16 * f < N) C[n + 16 * f] = gated(out[f], out[f + NF / 2]);
+        for (int f = 0; f < NF / 2; f++)
+          if (kw == 0 && r < 4 && n + 16 * f < N) C[n + 16 * f] = gated(out[f], out[f + NF / 2]);
+      }
     } else {
 #pragma unroll
       for (int f = 0; f < NF; f++)
@@ -274,7 +343,7 @@ template <int SRC, int NF, bool GATED>
 static hipError_t launch_rows(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N, int64_t K, int KW,
                               int waves, float* C, uint8_t* codes, uint8_t* scales, const MxRow& R) {
   constexpr int kTile = GATED ? 8 * NF : 16 * NF;
-  const int lds = std::max(SRC == kCodes ? 0 : waves * kUnitLds, rows_sums(NF, waves)) + (int)(waves / KW * 16 * NF * (K / kMxBlock)) + 16;
+  const int lds = std::max(SRC == kCodes ? 0 : waves * kUnitLds, rows_sums(NF, waves)) + (GATED ? 2 : 1) * whole_16((int)(waves / KW * kTile * (K / kMxBlock)));
   const auto kernel = mx_rows_kernel<SRC, NF, GATED>;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
   if (e != hipSuccess) return e;
@@ -306,8 +375,8 @@ __global__ __launch_bounds__(512, UPW * NF <= 4 ? 4 : 2) void mx_row_tiles_kerne
     const int n0 = min(tile, tiles - 1) * rows + fw * kTile;
 #pragma unroll
     for (int f = 0; f < NF; f++) {
-      const int n = min(n0 + 16 * (GATED ? f % (NF / 2) : f) + r, N - 1);
-      row[f] = W + ((GATED && f >= NF / 2 ? (int64_t)N : 0) + n) * nb * 16;
+      const TileRow t = tile_row<NF, GATED>(f, r);
+      row[f] = W + ((t.up ? (int64_t)N : 0) + min(n0 + t.n, N - 1)) * nb * 16;
     }
   };
   // (both halves of a row's 128 bytes one after the other, and not past the caches: the second finds the line there)
@@ -322,7 +391,7 @@ __global__ __launch_bounds__(512, UPW * NF <= 4 ? 4 : 2) void mx_row_tiles_kerne
 #pragma unroll
       for (int f = 0; f < NF; f++) ask(j, f);
   };
-  // scales of a tile, 16 bytes a thread (the launcher sees to it that the run is no more than 512 of those, and whole ones)
+  // scales of a tile, 16 bytes a thread (the launcher sees to it that the run is no more than 512 of those, and whole ones: rows * nb % 16 == 0, N % 16 == 0)
   any16 sc[GATED ? 2 : 1];
   const auto ask_scales = [&](int tile) {
     const int64_t total = (int64_t)N * nb, at = min((int64_t)min(tile, tiles - 1) * run_bytes + min(16 * tid, run_bytes - 16), total - 16);
@@ -408,7 +477,8 @@ __global__ __launch_bounds__(512, UPW * NF <= 4 ? 4 : 2) void mx_row_tiles_kerne
       }
 #pragma unroll
       for (int f = 0; f < NF; f++) {
-        const int in_run = (GATED && f >= NF / 2 ? run_bytes : 0) + (fw * kTile + 16 * (GATED ? f % (NF / 2) : f) + r) * nb;
+        const TileRow t = tile_row<NF, GATED>(f, r);
+        const int in_run = (t.up ? run_bytes : 0) + (fw * kTile + t.n) * nb;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
           const int b = 8 * (kw + j * KW) + 4 * h + g, ws = b < nb ? run[in_run + b] : 0;
@@ -429,17 +499,17 @@ __global__ __launch_bounds__(512, UPW * NF <= 4 ? 4 : 2) void mx_row_tiles_kerne
     // a row's sums over the KW wavefronts, one row a thread
     if (tid < FW * NF * 16) {
       const int w = tid / (NF * 16), f = tid / 16 % NF, i = tid & 15;
-      const auto sum = [&](int ff) {
-        float v = part[(w * KW * NF + ff) * 16 + i];
-        for (int k = 1; k < KW; k++) v += part[((w * KW + k) * NF + ff) * 16 + i];
+      const auto sum = [&](int i) {
+        float v = part[(w * KW * NF + f) * 16 + i];
+        for (int k = 1; k < KW; k++) v += part[((w * KW + k) * NF + f) * 16 + i];
         return v * inv;
       };
+      const int n = tile * rows + w * kTile + 16 * f + i;
       if constexpr (GATED) {
-        const int n = tile * rows + w * kTile + 16 * f + i;
-        if (f < NF / 2 && n < N) y[n] = gated(sum(f), sum(f + NF / 2));
+        static_assert(NF == 1, "gate rows in the lower half of a tile");
+        if (i < 8 && n < N) y[n] = gated(sum(i), sum(i + 8));
       } else {
-        const int n = tile * rows + w * kTile + 16 * f + i;
-        if (n < N) y[n] = sum(f);
+        if (n < N) y[n] = sum(i);
       }
     }
     tile = next;
@@ -470,16 +540,13 @@ template <int SRC, bool GATED>
 static hipError_t launch_row(const uint8_t* W, const uint8_t* sw, int64_t N, int64_t K, float* y, const MxRow& R) {
   const int64_t nb = K / kMxBlock, units = (nb + 7) / 8, cus = cu_count();
   const int KW = units <= 1 ? 1 : units <= 2 ? 2 : units <= 4 ? 4 : 8;
-  const int64_t rows = 16 * (8 / KW);          // of a tile, gate rows if gated
-  if (units <= 16 && N % 16 == 0 && N > 4 * cus * rows && rows * nb >= 16) {
-    constexpr int NF = GATED ? 2 : 1;
-    return (units <= KW ? launch_row_tiles<SRC, NF, GATED, 1> : launch_row_tiles<SRC, NF, GATED, 2>)(W, sw, N, K, KW, 2, y, R);
-  }
+  const int64_t rows = (GATED ? 8 : 16) * (8 / KW);          // of a tile, gate rows if gated
+  if constexpr (SRC != kMerged)
+    if (units <= 16 && N % 16 == 0 && N > 4 * cus * rows && rows * nb % 16 == 0)
+      return (units <= KW ? launch_row_tiles<SRC, 1, GATED, 1> : launch_row_tiles<SRC, 1, GATED, 2>)(W, sw, N, K, KW, 2, y, R);
   const int waves = units <= 12 ? 8 : 16, kw = units <= 8 ? KW : waves;
-  if constexpr (GATED) return launch_rows<SRC, 2, true>(nullptr, nullptr, W, sw, 1, N, K, kw, waves, y, nullptr, nullptr, R);
-  else
-    return (N > 16 * cus && nb <= 1024 ? launch_rows<SRC, 2, false> : launch_rows<SRC, 1, false>)(nullptr, nullptr, W, sw, 1, N, K, kw, waves, y, nullptr,
-                                                                                               nullptr, R);
+  const bool two = (GATED ? 2 : 1) * N > 16 * cus && nb <= 1024;
+  return (two ? launch_rows<SRC, 2, GATED> : launch_rows<SRC, 1, GATED>)(nullptr, nullptr, W, sw, 1, N, K, kw, waves, y, nullptr, nullptr, R);
 }
 
 bool mx_few_rows_fit(int64_t N, int64_t K, bool gated) {
@@ -505,8 +572,20 @@ int tlhip_gemv_mxfp4(const void* a, const void* codes, const void* scales, void*
   TLHIP_REQUIRE_READY();
   const char* who = "tlhip_gemv_mxfp4";
   if (const int rc = check_mx_product(who, a, scales, codes, scales, y, 1, N, K)) return rc;
-  const MxRow R{static_cast<const float*>(a), nullptr, nullptr, nullptr, 0.f};
+  const MxRow R{static_cast<const float*>(a), nullptr, nullptr, nullptr, 0.f, 0, 0, 0};
   const hipError_t e = launch_row<kFloat, false>(bytes(codes), bytes(scales), N, K, static_cast<float*>(y), R);
+  if (e != hipSuccess) return hip_fail(e, who);
+  TLHIP_CHECK_LAUNCH(TLHIP_C_GEMV_MXFP4);
+}
+
+int tlhip_gemv_mxfp4_attn(const void* parts, int64_t n_parts, int64_t heads, int64_t head_dim, const void* codes, const void* scales, void* y,
+                          int64_t N, int64_t K) {
+  TLHIP_REQUIRE_READY();
+  const char* who = "tlhip_gemv_mxfp4_attn";
+  if (const int rc = check_mx_product(who, parts, scales, codes, scales, y, 1, N, K)) return rc;
+  if (const int rc = check_attn_merge(parts, n_parts, heads, head_dim, K, who)) return rc;
+  const MxRow R{static_cast<const float*>(parts), nullptr, nullptr, nullptr, 0.f, (int)n_parts, (int)heads, (int)head_dim};
+  const hipError_t e = launch_row<kMerged, false>(bytes(codes), bytes(scales), N, K, static_cast<float*>(y), R);
   if (e != hipSuccess) return hip_fail(e, who);
   TLHIP_CHECK_LAUNCH(TLHIP_C_GEMV_MXFP4);
 }
@@ -517,7 +596,8 @@ static int normed(const char* who, const void* x, const void* delta, const void*
   if (!norm_w) return fail(TLHIP_EINVAL, "%s: null pointer", who);
   if (!aligned16(delta) || !aligned16(norm_w) || !aligned16(xout)) return fail(TLHIP_EINVAL, "%s: delta, norm_w and xout must be 16-byte aligned", who);
   if (xout && (xout == x || xout == delta)) return fail(TLHIP_EINVAL, "%s: xout must not alias x or delta", who);
-  const MxRow R{static_cast<const float*>(x), static_cast<const float*>(delta), static_cast<const float*>(norm_w), static_cast<float*>(xout), eps};
+  const MxRow R{static_cast<const float*>(x), static_cast<const float*>(delta), static_cast<const float*>(norm_w), static_cast<float*>(xout), eps,
+                0, 0, 0};
   const hipError_t e = (gate ? launch_row<kNormed, true> : launch_row<kNormed, false>)(bytes(codes), bytes(scales), N, K, static_cast<float*>(y), R);
   if (e != hipSuccess) return hip_fail(e, who);
   TLHIP_CHECK_LAUNCH(TLHIP_C_GEMV_MXFP4);

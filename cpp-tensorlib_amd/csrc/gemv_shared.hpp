@@ -184,6 +184,7 @@ __device__ __forceinline__ float wave_sum_rows(float (&a)[R], int lane) {
 //   kGeglu:  as kGateUp with y[i] = gelu_tanh(g + gu_bias[i]) * (u + gu_bias[N/2 + i]).
 enum { kPlain = 0, kSwiglu = 1, kRmsnorm = 2, kAttnMerge = 3, kPostnorm = 4, kPostnormLong = 5, kMixMerge = 6 };
 constexpr int kMergeMax = 16;  // splits the kAttnMerge producer takes (its lanes per head)
+int check_attn_merge(const void* parts, int64_t n_parts, int64_t heads, int64_t D, int64_t K, const char* who);
 constexpr int kMixMergeRow = 20480;   // columns of x that it takes: as many as 1024 threads ask for up front
 constexpr int kMixMergeMax = 8;  // splits the kMixMerge producer takes (one merge_group, its registers)
 enum { kStore = 0, kGateUp = 1, kGeglu = 2 };

@@ -186,6 +186,7 @@ struct api {
   int (*dequantize_mxfp8)(const void*, const void*, void*, int, int64_t, int64_t) = nullptr;
   int (*rmsnorm_res_mxfp8)(const void*, const void*, int64_t, const void*, void*, void*, void*, int64_t, float, int64_t) = nullptr;
   int (*gemv_mxfp4)(const void*, const void*, const void*, void*, int64_t, int64_t) = nullptr;
+  int (*gemv_mxfp4_attn)(const void*, int64_t, int64_t, int64_t, const void*, const void*, void*, int64_t, int64_t) = nullptr;
   int (*gemv_mxfp4_rmsnorm)(const void*, const void*, const void*, void*, const void*, const void*, void*, int64_t, int64_t,
                             float) = nullptr;
   int (*gemv_mxfp4_rmsnorm_gateup)(const void*, const void*, const void*, void*, const void*, const void*, void*, int64_t, int64_t,
@@ -436,7 +437,7 @@ struct context {
               bind(f.quantize_mxfp4, "tlhip_quantize_mxfp4") && bind(f.quantize_mxfp8, "tlhip_quantize_mxfp8") &&
               bind(f.dequantize_mxfp4, "tlhip_dequantize_mxfp4") && bind(f.dequantize_mxfp8, "tlhip_dequantize_mxfp8") &&
               bind(f.rmsnorm_res_mxfp8, "tlhip_rmsnorm_res_mxfp8") && bind(f.gemv_mxfp4, "tlhip_gemv_mxfp4") &&
-              bind(f.gemv_mxfp4_rmsnorm, "tlhip_gemv_mxfp4_rmsnorm") &&
+              bind(f.gemv_mxfp4_attn, "tlhip_gemv_mxfp4_attn") && bind(f.gemv_mxfp4_rmsnorm, "tlhip_gemv_mxfp4_rmsnorm") &&
               bind(f.gemv_mxfp4_rmsnorm_gateup, "tlhip_gemv_mxfp4_rmsnorm_gateup") &&
               bind(f.gemm_mxfp4_nt, "tlhip_gemm_mxfp4_nt") && bind(f.gemm_mxfp4_nt_parts, "tlhip_gemm_mxfp4_nt_parts") &&
               bind(f.gemm_mxfp4_nt_swiglu, "tlhip_gemm_mxfp4_nt_swiglu") &&
@@ -1530,6 +1531,15 @@ inline bool gemv_mxfp4(void* a, void* codes, void* scales, void* y, int64_t N, i
   L.reads(a, codes, scales);
   L.writes(y);
   return L.sent(L.lib.gemv_mxfp4(a, codes, scales, y, N, K));
+}
+// The row is the attention's output, in its split partials
+inline bool gemv_mxfp4_attn(void* parts, int64_t n_parts, int64_t heads, int64_t head_dim, void* codes, void* scales, void* y, int64_t N,
+                            int64_t K) {
+  launch L;
+  if (!L.ok || (K % 32) != 0 || heads * head_dim != K) return false;
+  L.reads(parts, codes, scales);
+  L.writes(y);
+  return L.sent(L.lib.gemv_mxfp4_attn(parts, n_parts, heads, head_dim, codes, scales, y, N, K));
 }
 inline bool gemv_mxfp4_rmsnorm(void* x, void* delta, void* norm_w, void* xout, void* codes, void* scales, void* y, int64_t N,
                                int64_t K, float eps) {

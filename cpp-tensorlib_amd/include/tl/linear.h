@@ -46,7 +46,7 @@ inline bool gemv_attn(const linear& L, void* parts, int n_parts, int64_t heads, 
   if (L.fmt == wfmt::q4)
     return hip::gemv_q4_attn(parts, n_parts, heads, head_dim, L.w, static_cast<char*>(L.w) + L.N * L.K / 2, y, L.N,
                              L.K, kQ4Group);
-  if (L.fmt == wfmt::mxfp4) return false;   // no such form
+  if (L.fmt == wfmt::mxfp4) return hip::gemv_mxfp4_attn(parts, n_parts, heads, head_dim, L.w, L.block_scales(), y, L.N, L.K);
   return hip::gemv_bf16_row_attn(parts, n_parts, heads, head_dim, L.w, y, L.N, L.K);
 }
 

@@ -654,8 +654,7 @@ inline bool run_layers(model& M, void* x0, int64_t pos, void* logits_out = nullp
     if (!M.rope_tab) M.rope_tab = hip::alloc_device(d.head_dim * 4);
     ok &= M.rope_tab && hip::rope_table(M.rope_tab, d.head_dim, pos, d_pos, d.rope_base);
     // the attention's splits merged by the o-projection: decided once per step from the launch plan
-    // (an MXFP4 o-projection takes the merged row only)
-    const bool merge = M.fused_attn && M.merge_in_oproj && M.attn_partials && M.layers[0].wo.fmt != wfmt::mxfp4 &&
+    const bool merge = M.fused_attn && M.merge_in_oproj && M.attn_partials &&
                        hip::attn_parts_splits(d.n_q_heads, d.n_kv_heads, d_pos ? M.layers[0].cache.max_ctx : pos + 1,
                                               d.head_dim, M.layers[0].cache.kv_bf16) > 0;
     size_t marks = 0;

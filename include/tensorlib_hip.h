@@ -654,7 +654,10 @@ int tlhip_rmsnorm_res_mxfp8(const void* x, const void* parts, int64_t S, const v
 /* y[n] = sum_k a[k] W[n][k], a f32, W MXFP4 [N][K], f32 sums: the decode product. A number of a keeps its 24 bits down to 2^-24 of the
  * largest of its block of 32, below that an absolute error of 2^-48 of that (and of 2^-128); an infinity or a NaN in a makes every y NaN. */
 int tlhip_gemv_mxfp4(const void* a, const void* codes, const void* scales, void* y, int64_t N, int64_t K);
-/* The same with the producers of tlhip_gemv_q4_rmsnorm and tlhip_gemv_q4_rmsnorm_gateup, whose arguments these have. */
+/* The same with the producers of tlhip_gemv_q4_attn, tlhip_gemv_q4_rmsnorm and tlhip_gemv_q4_rmsnorm_gateup, whose arguments these
+ * have. */
+int tlhip_gemv_mxfp4_attn(const void* parts, int64_t n_parts, int64_t heads, int64_t head_dim, const void* codes, const void* scales, void* y,
+                          int64_t N, int64_t K);
 int tlhip_gemv_mxfp4_rmsnorm(const void* x, const void* delta, const void* norm_w, void* xout, const void* codes, const void* scales, void* y,
                              int64_t N, int64_t K, float eps);
 int tlhip_gemv_mxfp4_rmsnorm_gateup(const void* x, const void* delta, const void* norm_w, void* xout, const void* codes, const void* scales,
