@@ -528,19 +528,178 @@ static hipError_t launch_row_tiles(const uint8_t* W, const uint8_t* sw, int64_t 
   return hipGetLastError();
 }
 
-// Which kernel, by sizes (us so, and in the other forms):
+// The same product where the weight is small, in the vector unit: blocks of few rows, so that all CUs have some, and no digits to make. A
+// wavefront has RW rows of the weight (gated: half of them gate rows, and their up rows), 16 numbers of each in a lane, and every KW-th
+// 1024 of k. An element is widened times 2^-8 (so that sixteen products of it with any finite number stay in f32), products are
+// summed in one chain per lane and scaled by their block's power of two after that, which is exact. A row with an infinity or a
+// NaN gives NaN, as its digits do.
+// A plain row's numbers are read by each lane for itself (896 x 4864 3.9 us, staged in LDS by the block 4.0, 3584 x 3584 4.1 and 4.6); what
+// goes through a norm is three times as much to read, and staged (896 x 4864 4.3, each lane for itself 4.5; 3584 x 3584 5.6, 7.2).
+__device__ __forceinline__ int row_place(int i) { return i + (i >> 4); }       // of float4 i: what lanes read together is in different banks
+template <int SRC, int RW, bool GATED>
+__global__ __launch_bounds__(1024) void mx_row_small_kernel(const uint8_t* __restrict__ W, const uint8_t* __restrict__ sw, int N, int nb, int KW, int FW,
+                                                          float* __restrict__ y, const MxRow R) {
+  constexpr int kTile = GATED ? RW / 2 : RW;                   // features of a wavefront
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ float sums[16][RW + 2];                           // of rows, of the squares, NaN of a row that is not finite
+  float4* const staged = reinterpret_cast<float4*>(lds);
+  const int tid = threadIdx.x, lane = tid & 63, threads = 64 * KW * FW;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), fw = wave / KW, kw = wave - fw * KW;
+  const int K = nb * kMxBlock, n4 = K / 4, n0 = ((int)blockIdx.x * FW + fw) * kTile;
+  const float4 *x4 = reinterpret_cast<const float4*>(R.x), *d4 = reinterpret_cast<const float4*>(R.delta), *w4 = reinterpret_cast<const float4*>(R.norm_w);
+  constexpr int kPre = 2;                                      // of the numbers a thread stages, asked for ahead of the weights
+  float4 v[4], x[kPre], d[kPre], nw[kPre];
+  MergeIn in[kPre];
+  if constexpr (SRC == kMerged) {
+#pragma unroll
+    for (int p = 0; p < kPre; p++) in[p] = ask_merge(R, 4 * min(tid + p * threads, n4 - 1), lane);
+  }
+  if constexpr (SRC == kNormed) {
+#pragma unroll
+    for (int p = 0; p < kPre; p++) {
+      const int i = min(tid + p * threads, n4 - 1);
+      x[p] = x4[i];
+      d[p] = d4 ? d4[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+      nw[p] = w4[i];
+    }
+  }
+  uint2 w[RW];
+  uint32_t s[RW];
+  const auto ask = [&](int k) {
+    const int at = min(k, K - 16);
+    if constexpr (SRC == kFloat) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] = x4[at / 4 + j];
+    }
+#pragma unroll
+    for (int i = 0; i < RW; i++) {
+      const int64_t row = min(n0 + i % kTile, N - 1) + (i < kTile ? (int64_t)0 : (int64_t)N);
+      w[i] = *reinterpret_cast<const uint2*>(W + row * nb * 16 + at / 2);
+      s[i] = sw[row * nb + at / kMxBlock];
+    }
+  };
+  const int first = 1024 * kw + 16 * lane;
+  ask(first);
+  float ss = 0.f, bad = 0.f;
+  const auto look = [&](const float4 a) { bad = fmaf(a.x, 0.f, fmaf(a.y, 0.f, fmaf(a.z, 0.f, fmaf(a.w, 0.f, bad)))); };
+  if constexpr (SRC == kMerged) {
+    const auto stage = [&](int i, const float4 a) {
+      look(a);
+      staged[row_place(i)] = a;
+    };
+#pragma unroll
+    for (int p = 0; p < kPre; p++)
+      if (tid + p * threads < n4) stage(tid + p * threads, merged(R, in[p], lane));
+    for (int i = tid + kPre * threads; i < n4; i += threads) stage(i, merged(R, ask_merge(R, 4 * i, lane), lane));
+  }
+  if constexpr (SRC == kNormed) {
+    const auto stage = [&](int i, float4 a, const float4 b, const float4 c) {
+      if (d4) a = plus(a, b);
+      if (R.xout && blockIdx.x == 0) reinterpret_cast<float4*>(R.xout)[i] = a;
+      ss += (a.x * a.x + a.y * a.y) + (a.z * a.z + a.w * a.w);
+      a = make_float4(a.x * c.x, a.y * c.y, a.z * c.z, a.w * c.w);
+      look(a);
+      staged[row_place(i)] = a;
+    };
+#pragma unroll
+    for (int p = 0; p < kPre; p++)
+      if (tid + p * threads < n4) stage(tid + p * threads, x[p], d[p], nw[p]);
+    for (int i = tid + kPre * threads; i < n4; i += threads) stage(i, x4[i], d4 ? d4[i] : make_float4(0.f, 0.f, 0.f, 0.f), w4[i]);
+  }
+  if constexpr (SRC != kFloat) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // (the weights stay in flight)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+  float total[RW];
+#pragma unroll
+  for (int i = 0; i < RW; i++) total[i] = 0.f;
+  for (int k = first; k - 16 * lane < K; k += 1024 * KW) {
+    if (k != first) ask(k);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if constexpr (SRC != kFloat) v[j] = staged[row_place(min(k, K - 16) / 4 + j)];
+      else look(v[j]);
+    }
+#pragma unroll
+    for (int i = 0; i < RW; i++) {
+      float c = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        constexpr float kDown = 0.00390625f;
+        const uint32_t q = j < 2 ? w[i].x : w[i].y;
+        const v2f a = j & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, kDown, 2) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, kDown, 0);
+        const v2f b = j & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, kDown, 3) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, kDown, 1);
+        c = fmaf(v[j].x, a[0], fmaf(v[j].y, a[1], fmaf(v[j].z, b[0], fmaf(v[j].w, b[1], c))));
+      }
+      c = s[i] == 255u ? __uint_as_float(0x7fc00000u) : ldexpf(c, (int)s[i] - 119);
+      total[i] += k < K ? c : 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RW; i++) {
+    const float t = wave_sum(total[i]);
+    if (lane == 0) sums[wave][i] = t;
+  }
+  if constexpr (SRC == kNormed) ss = wave_sum(ss);
+  bad = wave_sum(bad);
+  if (lane == 0) {
+    sums[wave][RW] = ss;
+    sums[wave][RW + 1] = bad;
+  }
+  __syncthreads();
+  if (tid >= FW * kTile) return;
+  const int f = tid / kTile, n = (int)blockIdx.x * FW * kTile + tid;
+  const auto sum = [&](int wave, int count, int i) {
+    float t = sums[wave][i];
+    for (int k = 1; k < count; k++) t += sums[wave + k][i];
+    return t;
+  };
+  const float finite = sum(0, KW * FW, RW + 1), inv = SRC == kNormed ? 1.0f / sqrtf(sum(0, KW * FW, RW) / (float)K + R.eps) : 1.f;
+  const float a = (sum(f * KW, KW, tid % kTile) + finite) * inv;
+  if (n >= N) return;
+  if constexpr (GATED) y[n] = gated(a, (sum(f * KW, KW, tid % kTile + kTile) + finite) * inv);
+  else y[n] = a;
+}
+
+template <int SRC, int RW, bool GATED>
+static hipError_t launch_row_small(const uint8_t* W, const uint8_t* sw, int64_t N, int64_t K, int KW, int FW, float* y, const MxRow& R) {
+  const int64_t rows = FW * (GATED ? RW / 2 : RW);
+  const int lds = SRC != kFloat ? (int)(K / 4 + K / 64 + 1) * 16 : 0;
+  const auto kernel = mx_row_small_kernel<SRC, RW, GATED>;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 144 * 1024);
+  if (e != hipSuccess) return e;
+  kernel<<<dim3((unsigned)((N + rows - 1) / rows)), dim3(64 * KW * FW), lds, ctx().stream>>>(W, sw, (int)N, (int)(K / kMxBlock), KW, FW, y, R);
+  return hipGetLastError();
+}
+
+// Which kernel, by sizes (us so, and in the other forms; weights not in any cache; "gated" and "normed" as told, else plain):
+//   up to 20 2^20 elements (behind a producer 9 2^20, or 1024 rows, of up to 32768), K from 512: mx_row_small_kernel, a wavefront for every 1024 k
+//     (896 x 4864 3.9, mx_rows_kernel 4.4; 3584 x 3584 4.1, 4.6; 1000 x 18944 5.2, 9.2; beyond, 8192 x 3584 6.0, 5.7. Normed 896 x 4864 4.3,
+//     5.1; 9728 x 896 4.3, 4.5, gated 4.4, 4.8; 1000 x 18944 8.6, 12.0; beyond, 3584 x 3584 5.6, 5.1; 20000 x 512 5.0, 4.5). Four rows a
+//     wavefront (1000 x 18944 5.2, two 6.2; 3584 x 3584 4.1, 4.4), two where that makes no more blocks than there are CUs (normed
+//     896 x 4864 4.3, four 4.5); two sets of wavefronts a block share what is staged.
 //   more than 4 tiles of 16 rows for each CU, K up to 4096: mx_row_tiles_kernel (152064 x 3584 51.6, row by row 55.2; 37888 x 3584 14.8, 16.0;
 //     9728 x 896, 2.4 tiles: 4.2, 4.2);
 //   K up to 1024: as many wavefronts share a row's K as it has units of 256, in several sets (9728 x 896 in two of four 4.2, in eight 4.4;
 //     150000 x 64 in eight of one 4.8, in two of four 11.4);
 //   up to twelve units of 256 k: eight; beyond: sixteen (3584 x 18944 9.8; eight 10.8; 4608 x 3584 4.8; 5.2);
-//   32 rows a block from 4096 on, where that still makes more than half as many blocks as there are CUs (4608 x 3584 4.8, 16: 5.3;
-//     3584 x 18944 12.9, 16: 9.8), and while the scales of their rows leave room in LDS.
+//   32 rows a block where there are more tiles of 16 than CUs (4608 x 3584 5.1, 16: 5.9; gated 6.6, 8.8; 3584 x 18944 12.9, 16: 9.8), and while
+//     the scales of their rows leave room in LDS.
 template <int SRC, bool GATED>
 static hipError_t launch_row(const uint8_t* W, const uint8_t* sw, int64_t N, int64_t K, float* y, const MxRow& R) {
   const int64_t nb = K / kMxBlock, units = (nb + 7) / 8, cus = cu_count();
   const int KW = units <= 1 ? 1 : units <= 2 ? 2 : units <= 4 ? 4 : 8;
   const int64_t rows = (GATED ? 8 : 16) * (8 / KW);          // of a tile, gate rows if gated
+  const int64_t all = GATED ? 2 * N : N;                     // rows of the weight
+  if constexpr (SRC == kFloat) {
+    if (all * K <= (int64_t)20 << 20 && K >= 512) return launch_row_small<SRC, 4, false>(W, sw, N, K, (int)std::min<int64_t>(16, (K + 1023) / 1024), 1, y, R);
+  } else {
+    if ((all * K <= (int64_t)9 << 20 || all <= 4 * cus) && K >= 512 && K <= 32768) {
+      const int kw = (int)std::min<int64_t>(16, (K + 1023) / 1024), fw = kw <= 8 ? 2 : 1;
+      return (all <= 2 * fw * cus ? launch_row_small<SRC, 2, GATED> : launch_row_small<SRC, 4, GATED>)(W, sw, N, K, kw, fw, y, R);
+    }
+  }
   if constexpr (SRC != kMerged)
     if (units <= 16 && N % 16 == 0 && N > 4 * cus * rows && rows * nb % 16 == 0)
       return (units <= KW ? launch_row_tiles<SRC, 1, GATED, 1> : launch_row_tiles<SRC, 1, GATED, 2>)(W, sw, N, K, KW, 2, y, R);

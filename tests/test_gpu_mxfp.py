@@ -302,8 +302,7 @@ def test_gated_token_product_behind_a_norm(lib, ff, K, delta):
 @pytest.mark.parametrize("D,heads,S", [(64, 14, 16), (64, 14, 5), (128, 28, 8), (128, 2, 3), (64, 4, 1), (64, 2, 9), (128, 64, 7)])
 @pytest.mark.parametrize("N", [1, 130, 4640])
 def test_token_product_of_the_attentions_splits(lib, orc, D, heads, S, N):
-    """Made-up partials, some of splits without a key: the row that the bf16 product merges (through the identity, exactly), then the
-    plain decode product, bit for bit; and 64 bits. A split's weight e^(m - M), |m - M| up to 60, has 60 / ln 2 + 4 roundings (of the
+    """Made-up partials, some of splits without a key: the row that the bf16 product merges (through the identity, exactly) and 64 bits. A split's weight e^(m - M), |m - M| up to 60, has 60 / ln 2 + 4 roundings (of the
     argument, and of the exponential), in the sums above and below; each sum has one more for each split, the quotient one."""
     r, K = rng(D, heads, S, N), heads * D
     m = r.uniform(-30, 30, (heads, S)).astype(np.float32)
@@ -315,21 +314,20 @@ def test_token_product_of_the_attentions_splits(lib, orc, D, heads, S, N):
     part = lib.to_device(np.concatenate([m.ravel(), l.ravel(), acc.ravel()]))
     codes, scales = weight(r, N, K)
     wc, ws = upload_rows(lib, codes, scales, True)
-    x, y, two, eye = lib.empty(K), lib.empty(N), lib.empty(N), lib.to_device(orc.to_bf16(np.eye(K, dtype=np.float32)))
+    x, y, eye = lib.empty(K), lib.empty(N), lib.to_device(orc.to_bf16(np.eye(K, dtype=np.float32)))
     lib.gemv_bf16_row_attn(part, S, heads, D, eye, x, K, K)
-    lib.gemv_mxfp4(x, wc, ws, two, N, K)
     lib.gemv_mxfp4_attn(part, S, heads, D, wc, ws, y, N, K)
-    assert np.array_equal(y.numpy().view(np.uint32), two.numpy().view(np.uint32))
+    merged, W = x.numpy().astype(np.float64), mx.values(codes, scales, True)
+    assert np.all(np.abs(y.numpy() - W @ merged) <= product_bound(merged[None], W, K)[0])
     w64 = np.exp(m.astype(np.float64) - m.max(axis=1, keepdims=True))
     row = ((w64[:, :, None] * acc).sum(axis=1) / (w64 * l).sum(axis=1)[:, None]).reshape(K)
     size = ((w64[:, :, None] * np.abs(acc)).sum(axis=1) / (w64 * l).sum(axis=1)[:, None]).reshape(K)
-    W = mx.values(codes, scales, True)
     bound = (128 + K / 128 + 64 + 2 * (60 / np.log(2) + 4 + S) + 1) * 2.0 ** -24 * (np.abs(W) @ size)
     assert np.all(np.abs(y.numpy() - W @ row) <= bound)
     for S_, h_ in ((17 if D == 64 else 9, heads), (0, heads), (S, heads + 1)):
         with pytest.raises(Exception):
             lib.gemv_mxfp4_attn(part, S_, h_, D, wc, ws, y, N, K)
-    for b in (part, wc, ws, x, y, two, eye):
+    for b in (part, wc, ws, x, y, eye):
         b.free()
 
 
