@@ -3,6 +3,7 @@
 #include "mx_mfma.hpp"
 
 #include <algorithm>
+#include <initializer_list>
 
 namespace tlhip {
 
@@ -30,6 +31,7 @@ __device__ __forceinline__ uint32_t four_scales(const uint8_t* row, int b, int n
 struct MxTiles {
   int tokens, count;       // tiles of tokens, all tiles
   int parts, steps;        // K split: parts of so many steps of 128
+  int64_t apart;           // numbers of C from one part to the next
 };
 
 template <int WF, int WT, int NF, int NT, int WPE, bool GATED, bool WORDS>
@@ -157,7 +159,7 @@ __global__ __launch_bounds__(64 * WF * WT, WPE) void mx_tile_kernel(const uint8_
   for (int t = 0; t < NT; t++) {
     const int m = tt * TT + (wt * NT + t) * 16 + r;
     if constexpr (!GATED) {
-      float* out = C + ((int64_t)at.part * M + m) * N;
+      float* out = C + at.part * P.apart + (int64_t)m * N;
 #pragma unroll
       for (int f = 0; f < NF; f++)
         if (m < M) store_features(out, tf * TF + (wf * NF + f) * 16 + 4 * g, N, c[f][t]);
@@ -174,7 +176,7 @@ __global__ __launch_bounds__(64 * WF * WT, WPE) void mx_tile_kernel(const uint8_
 
 template <int WF, int WT, int NF, int NT, int WPE, bool GATED>
 static hipError_t launch_tiles(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N, int64_t K, int parts,
-                               float* C, uint8_t* codes, uint8_t* scales) {
+                               int64_t apart, float* C, uint8_t* codes, uint8_t* scales) {
   constexpr int TF = 16 * NF * WF / (GATED ? 2 : 1), TT = 16 * NT * WT;
   constexpr int lds = 2 * (16 * NF * WF * 68 + TT * 132);
   static_assert(lds <= 160 * 1024, "LDS");
@@ -184,6 +186,7 @@ static hipError_t launch_tiles(const uint8_t* A, const uint8_t* sa, const uint8_
   const int all = (int)((K + 127) / 128);
   P.steps = (all + parts - 1) / parts;
   P.parts = (all + P.steps - 1) / P.steps;
+  P.apart = apart;
   const int nb = (int)(K / kMxBlock);
   const bool words = nb % 4 == 0 && ((reinterpret_cast<uintptr_t>(sa) | reinterpret_cast<uintptr_t>(sw)) & 3) == 0;
   const auto kernel = words ? mx_tile_kernel<WF, WT, NF, NT, WPE, GATED, true> : mx_tile_kernel<WF, WT, NF, NT, WPE, GATED, false>;
@@ -197,9 +200,10 @@ static hipError_t launch_tiles(const uint8_t* A, const uint8_t* sa, const uint8_
 // ---- which tiles --------------------------------------------------------------------------------------------------------
 // Features x tokens of a tile and its blocks on a CU: 128 x 64 (four), 128 x 128 (three), 256 x 128 (two). A step takes `one` us plus
 // `more` for each block on a CU, as measured on products of 30 to 2048 rows by 896 x 4864 to 37888 x 3584; the launch that adds
-// parts up 2.2 us and their traffic at 3.5 TB/s. Over 54 products of those sizes (every tile, 1 to 16 parts) the choice takes 1.01
-// times the best one's time in the mean and 1.12 at worst. Both sides: 77 x 896 x 4864 8.7 us in 13 parts of 128 x 64, 23.9 in one;
-// 2048 x 37888 x 3584 in one part 422 us with 256 x 128, 427 with 128 x 128, 532 with 128 x 64.
+// parts up 2.2 us and their traffic at 3.5 TB/s. Over 54 products of those sizes the choice takes 1.01 times the best one's time in the mean
+// and 1.13 at worst. Both sides: 77 x 896 x 4864 8.7 us in 8 parts of 128 x 64, 23.9 in one; 2048 x 37888 x 3584 in one part 422 us with
+// 256 x 128, 427 with 128 x 128, 532 with 128 x 64. Numbers of parts that the eight dies do not share evenly are not tried (77 x 3584 x 18944 in 10
+// parts 30.4 us, in 8 23.5, in 12 26.2).
 struct MxPlan { int variant = 0, parts = 1; double us = 1e30; };
 static const struct { int features, tokens; double one, more; } kVariant[3] = {{128, 64, 0.35, 0.38}, {128, 128, 0.4, 0.72}, {256, 128, 0.9, 1.55}};
 
@@ -209,7 +213,8 @@ static MxPlan plan_tiles(int64_t M, int64_t N, int64_t K, int64_t max_parts, boo
   for (int v = 0; v < 3; v++) {
     const int64_t features = kVariant[v].features / (gated ? 2 : 1);
     const int64_t tiles = (N + features - 1) / features * ((M + kVariant[v].tokens - 1) / kVariant[v].tokens);
-    for (int64_t S = 1; S <= std::min<int64_t>(max_parts, 16) && (S == 1 || steps / S >= 2); S++) {
+    for (const int64_t S : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      if (S > 1 && (S > max_parts || steps / S < 2)) break;
       const int64_t each = (steps + S - 1) / S, parts = (steps + each - 1) / each;
       const double per_cu = std::max(0.5, (double)(tiles * parts) / (double)cus);
       double us = 3.0 + (double)each * (kVariant[v].one + kVariant[v].more * per_cu);
@@ -221,13 +226,49 @@ static MxPlan plan_tiles(int64_t M, int64_t N, int64_t K, int64_t max_parts, boo
 }
 
 static hipError_t launch_plan(const MxPlan& P, const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N,
-                              int64_t K, float* C, uint8_t* codes, uint8_t* scales) {
+                              int64_t K, int64_t apart, float* C, uint8_t* codes, uint8_t* scales) {
   if (codes) {
     const auto go = P.variant == 0 ? launch_tiles<1, 4, 8, 1, 4, true> : P.variant == 1 ? launch_tiles<1, 4, 8, 2, 3, true> : launch_tiles<2, 2, 8, 4, 2, true>;
-    return go(A, sa, W, sw, M, N, K, 1, C, codes, scales);
+    return go(A, sa, W, sw, M, N, K, 1, 0, C, codes, scales);
   }
   const auto go = P.variant == 0 ? launch_tiles<1, 4, 8, 1, 4, false> : P.variant == 1 ? launch_tiles<1, 4, 8, 2, 3, false> : launch_tiles<2, 2, 8, 4, 2, false>;
-  return go(A, sa, W, sw, M, N, K, P.parts, C, nullptr, nullptr);
+  return go(A, sa, W, sw, M, N, K, P.parts, apart, C, nullptr, nullptr);
+}
+
+// ---- a split K's parts ----------------------------------------------------------------------------------------------------
+// C = their sum, in their order
+__global__ __launch_bounds__(256) void mx_sum_kernel(const float4* __restrict__ part, float* __restrict__ C, int64_t total, int64_t apart4, int S) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (4 * i >= total) return;
+  const float4 a = sum_parts(S, [&](int s) { return part[s * apart4 + i]; });
+  if (4 * i + 4 <= total) {
+    *reinterpret_cast<float4*>(C + 4 * i) = a;
+  } else {
+    const float v[4] = {a.x, a.y, a.z, a.w};
+    for (int k = 0; 4 * i + k < total; k++) C[4 * i + k] = v[k];
+  }
+}
+
+// The gated activation of the sums, parts [S][M][gate | up], as MXFP8 rows: a lane has four features, eight lanes a block
+struct MxGateUp { float4 g, u; };
+__device__ __forceinline__ MxGateUp plus(const MxGateUp& a, const MxGateUp& b) { return MxGateUp{plus(a.g, b.g), plus(a.u, b.u)}; }
+__global__ __launch_bounds__(256) void mx_gate_sum_kernel(const float4* __restrict__ part, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                          int64_t M, int f4, int S) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= M * f4) return;                                     // (whole groups of eight lanes)
+  const int64_t m = i / f4, at = m * f4 + i, apart4 = M * 2 * f4;
+  const MxGateUp gu = sum_parts(S, [&](int s) { return MxGateUp{part[s * apart4 + at], part[s * apart4 + at + f4]}; });
+  float v[4] = {gated_fast(gu.g.x, gu.u.x), gated_fast(gu.g.y, gu.u.y), gated_fast(gu.g.z, gu.u.z), gated_fast(gu.g.w, gu.u.w)};
+  uint32_t big = max(max(magnitude(v[0]), magnitude(v[1])), max(magnitude(v[2]), magnitude(v[3])));
+  big = max(big, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)big, 0xB1, 0xf, 0xf, true));    // quad_perm [1,0,3,2]
+  big = max(big, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)big, 0x4E, 0xf, 0xf, true));    // quad_perm [2,3,0,1]
+  big = max(big, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)big, 0x141, 0xf, 0xf, true));   // row_half_mirror
+  const uint32_t s = mx_scale_of(big, kMx8Exp);
+  const float up = mx_up(min(s, 252u));
+#pragma unroll
+  for (int k = 0; k < 4; k++) v[k] = s == 255u ? 0.f : v[k] * up;
+  reinterpret_cast<uint32_t*>(codes)[i] = to_e4m3x4(v[0], v[1], v[2], v[3]);
+  if ((i & 7) == 0) scales[i >> 3] = (uint8_t)s;
 }
 
 }  // namespace tlhip
@@ -250,10 +291,9 @@ int tlhip_gemm_mxfp4_nt_parts(const void* acodes, const void* ascales, const voi
     *n_parts = 1;
     e = launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, static_cast<float*>(parts), nullptr, nullptr);
   } else {
-    // (parts of no whole number of 16 bytes would not be stored as such)
-    const MxPlan P = plan_tiles(M, N, K, N % 4 == 0 ? parts_bytes / (M * N * 4) : 1, false, false);
+    const MxPlan P = plan_tiles(M, N, K, parts_bytes / (M * N * 4), false, false);
     *n_parts = P.parts;
-    e = launch_plan(P, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, static_cast<float*>(parts), nullptr, nullptr);
+    e = launch_plan(P, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, M * N, static_cast<float*>(parts), nullptr, nullptr);
   }
   if (e != hipSuccess) return hip_fail(e, who);
   TLHIP_CHECK_LAUNCH(TLHIP_C_GEMM_MXFP4);
@@ -268,17 +308,20 @@ int tlhip_gemm_mxfp4_nt(const void* acodes, const void* ascales, const void* cod
   if (M <= kMxFewRows) {
     e = launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, static_cast<float*>(C), nullptr, nullptr);
   } else {
-    MxPlan P = plan_tiles(M, N, K, N % 4 == 0 ? 16 : 1, false, true);
+    MxPlan P = plan_tiles(M, N, K, 16, false, true);
+    const int64_t apart = (M * N + 3) & ~(int64_t)3;
     float* out = static_cast<float*>(C);
     if (P.parts > 1) {
-      out = static_cast<float*>(scratch((size_t)P.parts * M * N * 4));
+      out = static_cast<float*>(scratch((size_t)P.parts * apart * 4));
       if (!out) {            // (a recording may not grow it)
         P = plan_tiles(M, N, K, 1, false, true);
         out = static_cast<float*>(C);
       }
     }
-    e = launch_plan(P, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, out, nullptr, nullptr);
-    if (e == hipSuccess && P.parts > 1) launch_part_sum(out, static_cast<float*>(C), M, N, N, N, P.parts, 0);
+    e = launch_plan(P, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, apart, out, nullptr, nullptr);
+    if (e == hipSuccess && P.parts > 1)
+      mx_sum_kernel<<<dim3((unsigned)((apart / 4 + 255) / 256)), dim3(256), 0, ctx().stream>>>(reinterpret_cast<const float4*>(out), static_cast<float*>(C),
+                                                                                              M * N, apart / 4, P.parts);
   }
   if (e != hipSuccess) return hip_fail(e, who);
   TLHIP_CHECK_LAUNCH(TLHIP_C_GEMM_MXFP4);
@@ -292,10 +335,27 @@ int tlhip_gemm_mxfp4_nt_swiglu(const void* acodes, const void* ascales, const vo
   if (!act_scales) return fail(TLHIP_EINVAL, "%s: null pointer", who);
   if (!mx_row(ff)) return fail(TLHIP_EINVAL, "%s: ff must be a multiple of 32", who);
   uint8_t *qc = static_cast<uint8_t*>(act_codes), *qs = static_cast<uint8_t*>(act_scales);
-  const hipError_t e = M <= kMxFewRows && mx_few_rows_fit(ff, K, true)
-                           ? launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, ff, K, nullptr, qc, qs)
-                           : launch_plan(plan_tiles(M, ff, K, 1, true, false), bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, ff, K,
-                                         nullptr, qc, qs);
+  // Few tiles over a long K: gate and up products in parts, and a launch that adds them up and gates (us so, and in one launch: 282 x 32 x 11552
+  // 13.6, 67.6; 310 x 832 x 8128 29.9, 65.6). For up to 16 rows blocks of 16 features then, not of 32 gate and 32 up rows (12 x 32 x 10368 11.5, 16.3; 7 x
+  // 1792 x 5440 9.1, 11.7; 16 x 512 x 1536 7.7, 8.1; 1024 7.6, 7.9; 16 x 6144 x 3584, where blocks of 64 rows fill the CUs, 14.0, 11.3).
+  const bool few = M <= kMxFewRows;
+  const MxPlan one = plan_tiles(M, ff, K, 1, true, false);
+  MxPlan two = plan_tiles(M, 2 * ff, K, few ? 1 : 16, false, false);
+  if (two.parts == 1) two.us += 4.0 * (double)M * (double)ff * 4.0 / 3.5e6;
+  const bool apart = few ? !mx_few_rows_fit(ff, K, true) || (K >= 1536 && ff / kMxBlock <= cu_count() / 2) : two.us + 2.2 < one.us;
+  float* const parts = apart ? static_cast<float*>(scratch((size_t)two.parts * M * 2 * ff * 4)) : nullptr;    // (a recording may not grow it)
+  hipError_t e;
+  if (parts) {
+    e = few ? launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, 2 * ff, K, parts, nullptr, nullptr)
+            : launch_plan(two, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, 2 * ff, K, M * 2 * ff, parts, nullptr, nullptr);
+    if (e == hipSuccess)
+      mx_gate_sum_kernel<<<dim3((unsigned)((M * (ff / 4) + 255) / 256)), dim3(256), 0, ctx().stream>>>(reinterpret_cast<const float4*>(parts), qc, qs, M,
+                                                                                                       (int)(ff / 4), two.parts);
+  } else if (few && mx_few_rows_fit(ff, K, true)) {
+    e = launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, ff, K, nullptr, qc, qs);
+  } else {
+    e = launch_plan(one, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, ff, K, 0, nullptr, qc, qs);
+  }
   if (e != hipSuccess) return hip_fail(e, who);
   TLHIP_CHECK_LAUNCH(TLHIP_C_GEMM_MXFP4);
 }

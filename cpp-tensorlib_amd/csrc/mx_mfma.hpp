@@ -66,6 +66,16 @@ __device__ __forceinline__ v8i row_operand(const frag16& lo, const frag16& hi) {
   return v8i{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
 }
 
+// What gemv_shared.hpp's gated() is, on the hardware's exponential and reciprocal (1 ulp each): e^-g = 2^t, t = -g log2 e in two terms, the
+// lower one as the first two of its series; from t = 128 on 0. The reciprocal knows no subnormal numbers: it is of (1 + e^-g) / 4.
+// Thirteen instructions instead of more than thirty: 1280 x 4160 gated x 96 15.0 us instead of 17.4, 2048 x 18944 x 3584 422 instead of 431.
+__device__ __forceinline__ float gated_fast(float g, float u) {
+  const float t = g * -1.44269502f, r = fmaf(g, -1.92596299e-8f, fmaf(g, -1.44269502f, -t));
+  float e = __builtin_amdgcn_exp2f(t);
+  e = fabsf(t) < 128.f ? fmaf(e, r * 0.693147182f, e) : e;
+  return g * 0.25f * __builtin_amdgcn_rcpf(fmaf(e, 0.25f, 0.25f)) * u;
+}
+
 // Gated activations of a token, features 4 g .. 4 g + 3 of two tiles of 16 (gates g0, g1, up values u0, u1): a block of 32, the lanes
 // of one l % 16, as MXFP8
 __device__ __forceinline__ void store_gated(const v4f& g0, const v4f& g1, const v4f& u0, const v4f& u1, int g, bool live, uint8_t* codes,
@@ -74,8 +84,8 @@ __device__ __forceinline__ void store_gated(const v4f& g0, const v4f& g1, const 
   uint32_t big = 0;
 #pragma unroll
   for (int k = 0; k < 4; k++) {
-    v[k] = gated(g0[k], u0[k]);
-    v[4 + k] = gated(g1[k], u1[k]);
+    v[k] = gated_fast(g0[k], u0[k]);
+    v[4 + k] = gated_fast(g1[k], u1[k]);
     big = max(big, max(magnitude(v[k]), magnitude(v[4 + k])));
   }
   big = max(big, (uint32_t)__shfl_xor((int)big, 16, kWave));
@@ -91,10 +101,12 @@ __device__ __forceinline__ void store_gated(const v4f& g0, const v4f& g1, const 
   }
 }
 
-// Features n .. n + 3 of a token's row of N
+// Features n .. n + 3 of a token's row of N (whose address is a multiple of 16 bytes, or of 4 where N is no multiple of 4)
+typedef float any4f __attribute__((ext_vector_type(4), aligned(4)));
 __device__ __forceinline__ void store_features(float* row, int n, int N, const v4f& v) {
   if (n >= N) return;
   if ((N & 3) == 0) *reinterpret_cast<v4f*>(row + n) = v;
+  else if (n + 4 <= N) *reinterpret_cast<any4f*>(row + n) = v;
   else
     for (int k = 0; k < 4; k++)
       if (n + k < N) row[n + k] = v[k];

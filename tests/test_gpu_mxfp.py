@@ -249,6 +249,72 @@ TOKENS = [(1, 32), (3, 64), (17, 96), (16, 512), (896, 896), (1000, 544), (33, 4
           (33280, 160), (16640, 3584), (16656, 1184), (16650, 1184), (40, 65536)]
 
 
+# few tiles over a long K: parts that are added up, and gated, by a launch of their own; rows of no whole number of 16 bytes
+@pytest.mark.parametrize("M,N,K", [(17, 1, 9408), (23, 3, 18496), (103, 1113, 2560), (200, 6, 3328), (130, 141, 4896), (33, 5, 65536)])
+def test_product_of_few_tiles(lib, M, N, K):
+    r = rng(71, M, N, K)
+    ac, asc = rows8(r, M, K)
+    wc, wsc = weight(r, N, K)
+    bufs = upload_rows(lib, ac, asc) + upload_rows(lib, wc, wsc, True)
+    out = guarded(lib, M * N * 4)
+    lib.gemm_mxfp4_nt(*bufs, out, M, N, K)
+    a, w = mx.values(ac, asc, False), mx.values(wc, wsc, True)
+    assert np.all(np.abs(taken(out, M * N * 4, np.float32, (M, N)) - a @ w.T) <= product_bound(a, w, K))
+    room = 16
+    parts = guarded(lib, room * M * N * 4)
+    parts.nbytes, nbytes = room * M * N * 4, parts.nbytes
+    n = lib.gemm_mxfp4_nt_parts(*bufs, parts, M, N, K)
+    parts.nbytes = nbytes
+    got = taken(parts, room * M * N * 4, np.float32, (room, M, N))[:n].astype(np.float64).sum(0)
+    assert n >= 1 and np.all(np.abs(got - a @ w.T) <= product_bound(a, w, K))
+    for b in bufs + (out, parts):
+        b.free()
+
+
+@pytest.mark.parametrize("M,ff,K", [(1, 32, 1536), (12, 32, 10368), (16, 96, 4096), (7, 4128, 2048), (19, 32, 9408), (282, 32, 11552), (130, 160, 2720), (40, 864, 3584), (5, 32, 65536)])
+def test_gated_product_of_few_tiles(lib, M, ff, K):
+    r = rng(73, M, ff, K)
+    ac, asc = rows8(r, M, K)
+    wc, wsc = weight(r, 2 * ff, K)
+    bufs = upload_rows(lib, ac, asc) + upload_rows(lib, wc, wsc, True)
+    oc, os_ = guarded(lib, M * ff), guarded(lib, M * ff // 32)
+    lib.gemm_mxfp4_nt_swiglu(*bufs, oc, os_, M, ff, K)
+    check_gated(taken(oc, M * ff, np.uint8, (M, ff)), taken(os_, M * ff // 32, np.uint8, (M, ff // 32)), mx.values(ac, asc, False), mx.values(wc, wsc, True), K)
+    for b in bufs + (oc, os_):
+        b.free()
+
+
+@pytest.mark.parametrize("g", [0.0, 1e-30, -1e-3, 5.0, -20.0, 60.0, -60.0, -86.0, 3e4, 3e38])
+def test_gate_of_small_and_large_numbers(lib, g):
+    """One row and K = 32: gate values g times 1, 2, 4 (by the weights' elements), up values of order one. Eight roundings of the gate's arithmetic."""
+    K, ff = 32, 32
+    a = np.zeros((1, K), np.float32)
+    a[0, 0], a[0, 1] = g, 1.0
+    ac, asc = mx.quantize(a, False)
+    w = np.zeros((2 * ff, K), np.float32)
+    w[:ff, 0] = np.resize([1, 2, 4, 1, 1], ff)
+    w[ff:, 1] = np.resize([1, 1.5, -3], ff)
+    if abs(g) > 1e3 or abs(g) < 1e-3:      # (the block has one scale: the gate's number alone)
+        w[ff:, 1], w[ff:, 0] = 0, 0.5
+    wc, wsc = mx.quantize(w, True)
+    bufs = upload_rows(lib, ac, asc) + upload_rows(lib, wc, wsc, True)
+    oc, os_ = guarded(lib, ff), guarded(lib, 1)
+    lib.gemm_mxfp4_nt_swiglu(*bufs, oc, os_, 1, ff, K)
+    gu = mx.values(ac, asc, False) @ mx.values(wc, wsc, True).T
+    with np.errstate(over="ignore", invalid="ignore"):
+        act = mx.swiglu(gu)
+    c, s = taken(oc, ff, np.uint8, (1, ff)), taken(os_, 1, np.uint8, (1, 1))
+    if np.abs(act).max() > 3.4e38:
+        assert s[0, 0] == 255 and not c.any()
+    else:
+        v = mx.values(c, s, False)
+        step = np.maximum(np.abs(act) * 2.0 ** -4, 2.0 ** (float(s[0, 0]) - 127 - 10))
+        top = 2.0 ** (float(s[0, 0]) - 127) * 448
+        assert np.all(np.abs(v - act) - np.maximum(np.abs(act) - top, 0) <= step + np.abs(act) * 2.0 ** -20 + 1e-37)
+    for b in bufs + (oc, os_):
+        b.free()
+
+
 @pytest.mark.parametrize("N,K", TOKENS)
 def test_token_product(lib, N, K):
     r = rng(8, N, K)
