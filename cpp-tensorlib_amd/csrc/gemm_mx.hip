@@ -198,27 +198,29 @@ static hipError_t launch_tiles(const uint8_t* A, const uint8_t* sa, const uint8_
 }
 
 // ---- which tiles --------------------------------------------------------------------------------------------------------
-// Features x tokens of a tile and its blocks on a CU: 128 x 64 (four), 128 x 128 (three), 256 x 128 (two). A step takes `one` us plus
-// `more` for each block on a CU, as measured on products of 30 to 2048 rows by 896 x 4864 to 37888 x 3584; the launch that adds
-// parts up 2.2 us and their traffic at 3.5 TB/s. Over 54 products of those sizes the choice takes 1.01 times the best one's time in the mean
-// and 1.13 at worst. Both sides: 77 x 896 x 4864 8.7 us in 8 parts of 128 x 64, 23.9 in one; 2048 x 37888 x 3584 in one part 422 us with
-// 256 x 128, 427 with 128 x 128, 532 with 128 x 64. Numbers of parts that the eight dies do not share evenly are not tried (77 x 3584 x 18944 in 10
+// Features x tokens of a tile. A step takes `one` us plus `more` for each block on a CU, as measured on products of 20 to 2048 rows by 896 x 4864
+// to 37888 x 3584; the launch that adds parts up 2.2 us and their traffic at 5.4 TB/s. Over 54 products of those sizes the choice takes 1.02
+// times the best one's time in the mean and 1.16 at worst. Both sides: 77 x 896 x 4864 7.6 us in 8 parts of 64 x 64, 8.7 of 128 x 64, 23.9 in
+// one; 512 x 18944 gated x 3584 116 us with 128 x 128, 132 with 256 x 128, 137 with 128 x 64, 162 with 64 x 64; 2048 so 422 with 256 x 128, 427
+// with 128 x 128, 532 with 128 x 64. Numbers of parts that the eight dies do not share evenly are not tried (77 x 3584 x 18944 in 10
 // parts 30.4 us, in 8 23.5, in 12 26.2).
 struct MxPlan { int variant = 0, parts = 1; double us = 1e30; };
-static const struct { int features, tokens; double one, more; } kVariant[3] = {{128, 64, 0.35, 0.38}, {128, 128, 0.4, 0.72}, {256, 128, 0.9, 1.55}};
+constexpr int kVariants = 4;
+static const struct { int features, tokens; double one, more; } kVariant[kVariants] = {
+    {64, 64, 0.194, 0.2475}, {128, 64, 0.342, 0.38}, {128, 128, 0.39, 0.72}, {256, 128, 0.66, 1.32}};
 
 static MxPlan plan_tiles(int64_t M, int64_t N, int64_t K, int64_t max_parts, bool gated, bool own_sum) {
   const int64_t cus = cu_count(), steps = (K + 127) / 128;
   MxPlan best;
-  for (int v = 0; v < 3; v++) {
+  for (int v = 0; v < kVariants; v++) {
     const int64_t features = kVariant[v].features / (gated ? 2 : 1);
     const int64_t tiles = (N + features - 1) / features * ((M + kVariant[v].tokens - 1) / kVariant[v].tokens);
     for (const int64_t S : {1, 2, 3, 4, 6, 8, 12, 16}) {
       if (S > 1 && (S > max_parts || steps / S < 2)) break;
       const int64_t each = (steps + S - 1) / S, parts = (steps + each - 1) / each;
-      const double per_cu = std::max(0.5, (double)(tiles * parts) / (double)cus);
-      double us = 3.0 + (double)each * (kVariant[v].one + kVariant[v].more * per_cu);
-      if (parts > 1) us += (own_sum ? 2.2 : 0.0) + (double)(2 * parts + 1) * (double)M * (double)N * 4.0 / 3.5e6;
+      const double per_cu = std::max(1.09, (double)(tiles * parts) / (double)cus);
+      double us = 2.25 + (double)each * (kVariant[v].one + kVariant[v].more * per_cu);
+      if (parts > 1) us += (own_sum ? 2.2 : 0.0) + (double)(2 * parts + 1) * (double)M * (double)N * 4.0 / 5.4e6;
       if (us < best.us) best = MxPlan{v, (int)parts, us};
     }
   }
@@ -228,10 +230,16 @@ static MxPlan plan_tiles(int64_t M, int64_t N, int64_t K, int64_t max_parts, boo
 static hipError_t launch_plan(const MxPlan& P, const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N,
                               int64_t K, int64_t apart, float* C, uint8_t* codes, uint8_t* scales) {
   if (codes) {
-    const auto go = P.variant == 0 ? launch_tiles<1, 4, 8, 1, 4, true> : P.variant == 1 ? launch_tiles<1, 4, 8, 2, 3, true> : launch_tiles<2, 2, 8, 4, 2, true>;
+    const auto go = P.variant == 0   ? launch_tiles<1, 4, 4, 1, 4, true>
+                    : P.variant == 1 ? launch_tiles<1, 4, 8, 1, 4, true>
+                    : P.variant == 2 ? launch_tiles<1, 4, 8, 2, 3, true>
+                                     : launch_tiles<2, 2, 8, 4, 2, true>;
     return go(A, sa, W, sw, M, N, K, 1, 0, C, codes, scales);
   }
-  const auto go = P.variant == 0 ? launch_tiles<1, 4, 8, 1, 4, false> : P.variant == 1 ? launch_tiles<1, 4, 8, 2, 3, false> : launch_tiles<2, 2, 8, 4, 2, false>;
+  const auto go = P.variant == 0   ? launch_tiles<1, 4, 4, 1, 4, false>
+                  : P.variant == 1 ? launch_tiles<1, 4, 8, 1, 4, false>
+                  : P.variant == 2 ? launch_tiles<1, 4, 8, 2, 3, false>
+                                   : launch_tiles<2, 2, 8, 4, 2, false>;
   return go(A, sa, W, sw, M, N, K, P.parts, apart, C, nullptr, nullptr);
 }
 
@@ -336,12 +344,12 @@ int tlhip_gemm_mxfp4_nt_swiglu(const void* acodes, const void* ascales, const vo
   if (!mx_row(ff)) return fail(TLHIP_EINVAL, "%s: ff must be a multiple of 32", who);
   uint8_t *qc = static_cast<uint8_t*>(act_codes), *qs = static_cast<uint8_t*>(act_scales);
   // Few tiles over a long K: gate and up products in parts, and a launch that adds them up and gates (us so, and in one launch: 282 x 32 x 11552
-  // 13.6, 67.6; 310 x 832 x 8128 29.9, 65.6). For up to 16 rows blocks of 16 features then, not of 32 gate and 32 up rows (12 x 32 x 10368 11.5, 16.3; 7 x
+  // 12.5, 55.9; 310 x 832 x 8128 26.5, 49.9). For up to 16 rows blocks of 16 features then, not of 32 gate and 32 up rows (12 x 32 x 10368 11.5, 16.3; 7 x
   // 1792 x 5440 9.1, 11.7; 16 x 512 x 1536 7.7, 8.1; 1024 7.6, 7.9; 16 x 6144 x 3584, where blocks of 64 rows fill the CUs, 14.0, 11.3).
   const bool few = M <= kMxFewRows;
   const MxPlan one = plan_tiles(M, ff, K, 1, true, false);
   MxPlan two = plan_tiles(M, 2 * ff, K, few ? 1 : 16, false, false);
-  if (two.parts == 1) two.us += 4.0 * (double)M * (double)ff * 4.0 / 3.5e6;
+  if (two.parts == 1) two.us += 4.0 * (double)M * (double)ff * 4.0 / 5.4e6;
   const bool apart = few ? !mx_few_rows_fit(ff, K, true) || (K >= 1536 && ff / kMxBlock <= cu_count() / 2) : two.us + 2.2 < one.us;
   float* const parts = apart ? static_cast<float*>(scratch((size_t)two.parts * M * 2 * ff * 4)) : nullptr;    // (a recording may not grow it)
   hipError_t e;
