@@ -199,7 +199,7 @@ static hipError_t launch_tiles(const uint8_t* A, const uint8_t* sa, const uint8_
 
 // ---- which tiles --------------------------------------------------------------------------------------------------------
 // Features x tokens of a tile. A step takes `one` us plus `more` for each block on a CU, as measured on products of 20 to 2048 rows by 896 x 4864
-// to 37888 x 3584; the launch that adds parts up 2.2 us and their traffic at 5.4 TB/s. Over 54 products of those sizes the choice takes 1.02
+// to 37888 x 3584; the launch that adds parts up 2.2 us and their traffic at 5.4 TB/s. Over 54 products of those sizes the choice takes 1.01
 // times the best one's time in the mean and 1.16 at worst. Both sides: 77 x 896 x 4864 7.6 us in 8 parts of 64 x 64, 8.7 of 128 x 64, 23.9 in
 // one; 512 x 18944 gated x 3584 116 us with 128 x 128, 132 with 256 x 128, 137 with 128 x 64, 162 with 64 x 64; 2048 so 422 with 256 x 128, 427
 // with 128 x 128, 532 with 128 x 64. Numbers of parts that the eight dies do not share evenly are not tried (77 x 3584 x 18944 in 10
@@ -207,7 +207,7 @@ static hipError_t launch_tiles(const uint8_t* A, const uint8_t* sa, const uint8_
 struct MxPlan { int variant = 0, parts = 1; double us = 1e30; };
 constexpr int kVariants = 4;
 static const struct { int features, tokens; double one, more; } kVariant[kVariants] = {
-    {64, 64, 0.194, 0.2475}, {128, 64, 0.342, 0.38}, {128, 128, 0.39, 0.72}, {256, 128, 0.66, 1.32}};
+    {64, 64, 0.194, 0.2475}, {128, 64, 0.342, 0.38}, {128, 128, 0.39, 0.72}, {256, 128, 0.8, 1.34}};
 
 static MxPlan plan_tiles(int64_t M, int64_t N, int64_t K, int64_t max_parts, bool gated, bool own_sum) {
   const int64_t cus = cu_count(), steps = (K + 127) / 128;
