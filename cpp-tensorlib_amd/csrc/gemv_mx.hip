@@ -541,7 +541,7 @@ __global__ __launch_bounds__(1024) void mx_row_small_kernel(const uint8_t* __res
                                                           float* __restrict__ y, const MxRow R) {
   constexpr int kTile = GATED ? RW / 2 : RW;                   // features of a wavefront
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ float sums[16][RW + 2];                           // of rows, of the squares, NaN of a row that is not finite
+  __shared__ float sums[16][RW + 1];                           // of rows; of the squares, and NaN for a row that is not finite
   float4* const staged = reinterpret_cast<float4*>(lds);
   const int tid = threadIdx.x, lane = tid & 63, threads = 64 * KW * FW;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), fw = wave / KW, kw = wave - fw * KW;
@@ -579,7 +579,7 @@ __global__ __launch_bounds__(1024) void mx_row_small_kernel(const uint8_t* __res
     }
   };
   const int first = 1024 * kw + 16 * lane;
-  ask(first);
+  if constexpr (SRC != kFloat) ask(first);                     // (ahead of the row's staging)
   float ss = 0.f, bad = 0.f;
   const auto look = [&](const float4 a) { bad = fmaf(a.x, 0.f, fmaf(a.y, 0.f, fmaf(a.z, 0.f, fmaf(a.w, 0.f, bad)))); };
   if constexpr (SRC == kMerged) {
@@ -615,7 +615,7 @@ __global__ __launch_bounds__(1024) void mx_row_small_kernel(const uint8_t* __res
 #pragma unroll
   for (int i = 0; i < RW; i++) total[i] = 0.f;
   for (int k = first; k - 16 * lane < K; k += 1024 * KW) {
-    if (k != first) ask(k);
+    if (SRC == kFloat || k != first) ask(k);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       if constexpr (SRC != kFloat) v[j] = staged[row_place(min(k, K - 16) / 4 + j)];
@@ -638,14 +638,12 @@ __global__ __launch_bounds__(1024) void mx_row_small_kernel(const uint8_t* __res
   }
 #pragma unroll
   for (int i = 0; i < RW; i++) {
-    const float t = wave_sum(total[i]);
+    const float t = wave_sum(SRC == kFloat ? total[i] + bad : total[i]);
     if (lane == 0) sums[wave][i] = t;
   }
-  if constexpr (SRC == kNormed) ss = wave_sum(ss);
-  bad = wave_sum(bad);
-  if (lane == 0) {
-    sums[wave][RW] = ss;
-    sums[wave][RW + 1] = bad;
+  if constexpr (SRC != kFloat) {
+    ss = wave_sum(ss + bad);
+    if (lane == 0) sums[wave][RW] = ss;
   }
   __syncthreads();
   if (tid >= FW * kTile) return;
@@ -655,10 +653,11 @@ __global__ __launch_bounds__(1024) void mx_row_small_kernel(const uint8_t* __res
     for (int k = 1; k < count; k++) t += sums[wave + k][i];
     return t;
   };
-  const float finite = sum(0, KW * FW, RW + 1), inv = SRC == kNormed ? 1.0f / sqrtf(sum(0, KW * FW, RW) / (float)K + R.eps) : 1.f;
-  const float a = (sum(f * KW, KW, tid % kTile) + finite) * inv;
+  const float row = SRC != kFloat ? sum(0, KW * FW, RW) : 0.f;                       // (of a merged row: 0 or NaN)
+  const float inv = SRC == kNormed ? 1.0f / sqrtf(row / (float)K + R.eps) : 1.f;
+  const float a = (sum(f * KW, KW, tid % kTile) + (SRC == kMerged ? row : 0.f)) * inv;
   if (n >= N) return;
-  if constexpr (GATED) y[n] = gated(a, (sum(f * KW, KW, tid % kTile + kTile) + finite) * inv);
+  if constexpr (GATED) y[n] = gated(a, sum(f * KW, KW, tid % kTile + kTile) * inv);
   else y[n] = a;
 }
 
