@@ -15,7 +15,7 @@ namespace tlhip {
 // from wherever it lies.
 // Bound by the matrix cores: each element is multiplied twice, as its large and its small half, so their ceiling is half the
 // formats' (about 1.9e15 products and sums a second at the clock that such a load leaves). 2048 x 37888 x 3584 with the gate takes
-// 424 us (1.31e15 a second), 512 x 3584 x 18944 66 us (1.05e15, two parts' traffic and their sum in it). The activations straight
+// 422 us (1.32e15 a second), 512 x 3584 x 18944 66 us (1.05e15, four parts' traffic and their sum in it). The activations straight
 // into registers took 484 us instead of 436; a third stage of LDS and raised wave priorities changed nothing.
 typedef uint32_t any4 __attribute__((aligned(1)));
 __device__ __forceinline__ uint32_t four_scales(const uint8_t* row, int b, int nb) {      // bytes b .. b + 3 of nb, 0 past them (b < nb)
@@ -182,7 +182,9 @@ static hipError_t launch_tiles(const uint8_t* A, const uint8_t* sa, const uint8_
   static_assert(lds <= 160 * 1024, "LDS");
   MxTiles P;
   P.tokens = (int)((M + TT - 1) / TT);
-  P.count = (int)((N + TF - 1) / TF) * P.tokens;
+  const int64_t count = (N + TF - 1) / TF * P.tokens;
+  if (count > (1 << 24) / (WF * WT)) return hipErrorInvalidValue;   // (a grid's x counts threads in 32 bits)
+  P.count = (int)count;
   const int all = (int)((K + 127) / 128);
   P.steps = (all + parts - 1) / parts;
   P.parts = (all + P.steps - 1) / P.steps;
@@ -342,6 +344,8 @@ int tlhip_gemm_mxfp4_nt_swiglu(const void* acodes, const void* ascales, const vo
   if (const int rc = check_mx_product(who, acodes, ascales, codes, scales, act_codes, M, ff, K)) return rc;
   if (!act_scales) return fail(TLHIP_EINVAL, "%s: null pointer", who);
   if (!mx_row(ff)) return fail(TLHIP_EINVAL, "%s: ff must be a multiple of 32", who);
+  if (act_codes == acodes || act_scales == ascales || act_codes == act_scales)
+    return fail(TLHIP_EINVAL, "%s: the activation must not be written over the rows", who);
   uint8_t *qc = static_cast<uint8_t*>(act_codes), *qs = static_cast<uint8_t*>(act_scales);
   // Few tiles over a long K: gate and up products in parts, and a launch that adds them up and gates (us so, and in one launch: 282 x 32 x 11552
   // 12.5, 55.9; 310 x 832 x 8128 26.5, 49.9). For up to 16 rows blocks of 16 features then, not of 32 gate and 32 up rows (12 x 32 x 10368 11.5, 16.3; 7 x

@@ -32,6 +32,7 @@ inline int check_mx_product(const char* who, const void* a, const void* sa, cons
   if (M <= 0 || N <= 0 || !mx_row(K)) return fail(TLHIP_EINVAL, "%s: need M, N > 0, K a positive multiple of 32", who);
   if (!aligned16(a) || !aligned16(W) || !aligned16(out)) return fail(TLHIP_EINVAL, "%s: elements and result must be 16-byte aligned", who);
   if (M > (1 << 20) || N > (1 << 24) || K > kMxMaxK) return fail(TLHIP_EUNSUPPORTED, "%s: M up to 2^20, N up to 2^24, K up to 65536", who);
+  if (M * N > (int64_t)1 << 37) return fail(TLHIP_EUNSUPPORTED, "%s: results of up to 2^37 numbers", who);
   return TLHIP_OK;
 }
 

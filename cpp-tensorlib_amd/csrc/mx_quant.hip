@@ -209,6 +209,7 @@ static int dequantize(const char* who, const void* codes, const void* scales, vo
   if (rows <= 0 || !mx_row(K)) return fail(TLHIP_EINVAL, "%s: need rows > 0, K a positive multiple of 32", who);
   if (!aligned16(codes) || !aligned16(dst)) return fail(TLHIP_EINVAL, "%s: codes and dst must be 16-byte aligned", who);
   if (rows > ((int64_t)1 << 50) / K) return fail(TLHIP_EUNSUPPORTED, "%s: too many elements", who);
+  if (dst == codes || dst == scales) return fail(TLHIP_EINVAL, "%s: dst must not be what it is read from", who);
   const int64_t eights = rows * K / 8;
   for (int64_t e0 = 0; e0 < eights; e0 += (int64_t)1 << 31) {
     const int64_t n = std::min<int64_t>(eights - e0, (int64_t)1 << 31);
@@ -238,6 +239,7 @@ int tlhip_quantize_mxfp4(const void* src, int src_type, void* codes, void* scale
   if (rows <= 0 || !mx_row(K)) return fail(TLHIP_EINVAL, "%s: need rows > 0, K a positive multiple of 32", who);
   if (!aligned16(src) || !aligned16(codes)) return fail(TLHIP_EINVAL, "%s: src and codes must be 16-byte aligned", who);
   if (rows > ((int64_t)1 << 50) / K) return fail(TLHIP_EUNSUPPORTED, "%s: too many elements", who);
+  if (src == codes || src == scales || codes == scales) return fail(TLHIP_EINVAL, "%s: src, codes and scales must not be the same", who);
   const int64_t eights = rows * K / 8;
   if (src_type == TLHIP_T_F32) launch_quantize<TLHIP_T_F32, true>(src, codes, scales, eights);
   else if (src_type == TLHIP_T_F16) launch_quantize<TLHIP_T_F16, true>(src, codes, scales, eights);
@@ -252,6 +254,7 @@ int tlhip_quantize_mxfp8(const void* x, void* codes, void* scales, int64_t rows,
   if (rows <= 0 || !mx_row(K)) return fail(TLHIP_EINVAL, "%s: need rows > 0, K a positive multiple of 32", who);
   if (!aligned16(x) || !aligned16(codes)) return fail(TLHIP_EINVAL, "%s: x and codes must be 16-byte aligned", who);
   if (rows > ((int64_t)1 << 50) / K) return fail(TLHIP_EUNSUPPORTED, "%s: too many elements", who);
+  if (x == codes || x == scales || codes == scales) return fail(TLHIP_EINVAL, "%s: x, codes and scales must not be the same", who);
   launch_quantize<TLHIP_T_F32, false>(x, codes, scales, rows * K / 8);
   TLHIP_CHECK_LAUNCH(TLHIP_C_QUANTIZE_MX);
 }
@@ -272,11 +275,13 @@ int tlhip_rmsnorm_res_mxfp8(const void* x, const void* parts, int64_t S, const v
   const char* who = "tlhip_rmsnorm_res_mxfp8";
   if (!x || !w || !codes || !scales || (S > 0 && !parts)) return fail(TLHIP_EINVAL, "%s: null pointer", who);
   if (rows <= 0 || !mx_row(n)) return fail(TLHIP_EINVAL, "%s: need rows > 0, n a positive multiple of 32", who);
-  if (S < 0 || S > 64 || n > kNormMax || rows > 0x7fffffff)
-    return fail(TLHIP_EUNSUPPORTED, "%s: at most 64 parts and rows of 32768", who);
+  if (S < 0 || S > 64 || n > kNormMax || rows > (1 << 20))
+    return fail(TLHIP_EUNSUPPORTED, "%s: at most 64 parts, 2^20 rows of 32768", who);
   if (!aligned16(x) || !aligned16(parts) || !aligned16(w) || !aligned16(xout) || !aligned16(codes))
     return fail(TLHIP_EINVAL, "%s: x, parts, w, xout and codes must be 16-byte aligned", who);
   if (S > 0 && xout == parts) return fail(TLHIP_EINVAL, "%s: xout must not alias the parts", who);
+  if (codes == x || codes == xout || codes == w || codes == scales || (S > 0 && codes == parts) || scales == x || scales == xout)
+    return fail(TLHIP_EINVAL, "%s: codes and scales must not be x, xout, w, the parts or the same", who);
   const int64_t eights = n / 8, V = eights <= 1024 ? 1 : eights <= 2048 ? 2 : 4, threads = ((eights + V - 1) / V + 63) / 64 * 64;
   const auto kernel = V == 1 ? rmsnorm_mxfp8_kernel<1> : V == 2 ? rmsnorm_mxfp8_kernel<2> : rmsnorm_mxfp8_kernel<4>;
   kernel<<<dim3((unsigned)rows), dim3((unsigned)threads), 0, ctx().stream>>>(

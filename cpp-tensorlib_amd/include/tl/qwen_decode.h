@@ -807,7 +807,7 @@ inline bool prefill_reserve(model& M, int64_t T) {
 
 // Chunks over MXFP4 weights (no reference counterpart): every product reads MXFP8 rows, which its producer writes - the norms,
 // the gate's epilogue, and one rounding of the attention's rows; the residual, the caches and the attention stay f32. The rows lie
-// in scratch that these chunks have no other use for. Decode steps take f32 rows, so a token's logits differ between the
+// in scratch that these chunks have no other use for. There is this one sequence: fused_prefill has no effect. Decode steps take f32 rows, so a token's logits differ between the
 // two by the rounding of the chunk's activations.
 inline bool prefill_layers_mx(model& M, int64_t T) {
   const dims& d = M.d;

@@ -637,8 +637,9 @@ int tlhip_latent_attn_run(const void* u, int64_t ldu, const void* q, int64_t ldq
  * scales [rows][K/32] bytes in both. Rows are dense and K is a multiple of 32, so rows of two matrices of the same K can be stacked.
  * Rounding a block: s = floor(log2(largest magnitude)) + 127 - 2 (MXFP4) or - 8 (MXFP8), at least 0; every element is the value
  * over 2^(s - 127), rounded to nearest, ties to even, magnitudes beyond the type's largest becoming that. A block that holds
- * an infinity or a NaN gets the scale 255 and elements 0. Elements must be 16-byte aligned, scales need no alignment. Products take
- * M up to 2^20, N up to 2^24 and K up to 65536. */
+ * an infinity or a NaN gets the scale 255 and elements 0. What is written must not overlap what is read. Elements must be
+ * 16-byte aligned, scales need no alignment. Products take M up to 2^20, N up to 2^24, K up to 65536 and results of up to
+ * 2^37 numbers. */
 /* rows of TLHIP_T_F32, _F16 or _BF16 as a model file holds them -> MXFP4 */
 int tlhip_quantize_mxfp4(const void* src, int src_type, void* codes, void* scales, int64_t rows, int64_t K);
 /* f32 rows -> MXFP8 */
@@ -648,7 +649,7 @@ int tlhip_dequantize_mxfp4(const void* codes, const void* scales, void* dst, int
 int tlhip_dequantize_mxfp8(const void* codes, const void* scales, void* dst, int dst_type, int64_t rows, int64_t K);
 /* xout = x + (parts[0] + ... + parts[S-1]) in f32, ascending, parts [S][rows][n] (S = 0: none, parts may be NULL);
  * h = xout / sqrt(mean(xout^2) + eps) * w in 64 bits, rounded to f32, then to MXFP8. xout may be NULL, or x; not the parts.
- * n up to 32768, S up to 64. A row's bytes do not depend on how many rows there are. */
+ * n up to 32768, S up to 64, rows up to 2^20. A row's bytes do not depend on how many rows there are. */
 int tlhip_rmsnorm_res_mxfp8(const void* x, const void* parts, int64_t S, const void* w, void* xout, void* codes, void* scales,
                             int64_t n, float eps, int64_t rows);
 /* y[n] = sum_k a[k] W[n][k], a f32, W MXFP4 [N][K], f32 sums: the decode product. A number of a keeps its 24 bits down to 2^-24 of the

@@ -527,6 +527,61 @@ def test_layer_of_a_prompt(lib, M):
     assert np.array_equal(hc.numpy().reshape(M, E), want[0]) and np.array_equal(hs.numpy().reshape(M, -1), want[1])
 
 
+@pytest.mark.parametrize("N,K", [(131136, 65536), ((1 << 21) + 64, 4096)])
+def test_weights_beyond_four_gigabytes(lib, N, K):
+    """Rows of ones, the last 40 of them random: every kernel's offsets into a weight of more than 2^32 bytes."""
+    r, tail = rng(81, N), 40
+    codes, scales = weight(r, tail, K)
+    wc, ws = lib.empty_bytes(N * K // 2), lib.empty_bytes(N * K // 32)
+    lib._chk(lib.c.tlhip_fill_u32(wc.ptr, 0x22222222, N * K // 8))
+    lib._chk(lib.c.tlhip_fill_u32(ws.ptr, 0x7f7f7f7f, N * K // 128))
+    packed = np.ascontiguousarray(mx.pack(codes))
+    lib._chk(lib.c.tlhip_memcpy_h2d(wc.ptr + (N - tail) * K // 2, packed.ctypes.data, packed.nbytes))
+    scales = np.ascontiguousarray(scales)
+    lib._chk(lib.c.tlhip_memcpy_h2d(ws.ptr + (N - tail) * K // 32, scales.ctypes.data, scales.nbytes))
+    w = np.concatenate([np.ones((1, K)), mx.values(codes, scales, True)])
+    a = activations(r, 17, K)
+    x, y = lib.to_device(a[0]), lib.empty(N)
+    lib.gemv_mxfp4(x, wc, ws, y, N, K)
+    want, bound = (a[:1].astype(np.float64) @ w.T)[0], product_bound(a[:1].astype(np.float64), w, K)[0]
+    got = y.numpy()
+    assert np.all(np.abs(got[:N - tail] - want[0]) <= bound[0]) and np.all(np.abs(got[N - tail:] - want[1:]) <= bound[1:])
+    ac, asc = mx.quantize(a, False)
+    av = mx.values(ac, asc, False)
+    want, bound = av @ w.T, product_bound(av, w, K)
+    da, out = upload_rows(lib, ac, asc), lib.empty((17, N))
+    for M in (3, 17):
+        lib.gemm_mxfp4_nt(*da, wc, ws, out, M, N, K)
+        got = out.numpy().reshape(17, N)[:M]
+        assert np.all(np.abs(got[:, :N - tail] - want[:M, :1]) <= bound[:M, :1])
+        assert np.all(np.abs(got[:, N - tail:] - want[:M, 1:]) <= bound[:M, 1:])
+    ff = N // 2                                  # gate rows of ones, up rows of ones and the random ones
+    oc, os_ = lib.empty_bytes(17 * ff), lib.empty_bytes(17 * ff // 32)
+    up = 2.0 ** -14                              # (sums of thousands of numbers of order one: a row small enough for the gate)
+    ac, asc = mx.quantize(a * np.float32(up), False)
+    av = mx.values(ac, asc, False)
+    for b in da:
+        b.free()
+    da = upload_rows(lib, ac, asc)
+    gu = av @ w.T
+    bound = product_bound(av, w, K)
+    for M in (3, 17):
+        lib.gemm_mxfp4_nt_swiglu(*da, wc, ws, oc, os_, M, ff, K)
+        v = mx.values(oc.numpy(np.uint8)[:M * ff].reshape(M, ff)[:, ff - 64:], os_.numpy(np.uint8)[:M * ff // 32].reshape(M, ff // 32)[:, -2:], False)
+        g, u = gu[:M, :1], np.concatenate([np.repeat(gu[:M, :1], 64 - tail, 1), gu[:M, 1:]], 1)
+        act = mx.swiglu(np.concatenate([np.repeat(g, 64, 1), u], 1))
+        bu = np.concatenate([np.repeat(bound[:M, :1], 64 - tail, 1), bound[:M, 1:]], 1)
+        off = 1.1 * np.abs(u) * bound[:M, :1] + np.abs(act / np.where(u == 0, 1, u)) * bu + np.abs(act) * 2.0 ** -20 + 1e-37
+        top = np.abs(act).reshape(M, 2, 32).max(-1).repeat(32, 1)
+        # one rounding of an element: half a step of its own, or 2^-10 of the scale, which is at most 2^-8 of the largest;
+        # what lies in [448, 512) times the scale became 448, at most an eighth off
+        step = np.maximum(np.abs(act) * 2.0 ** -4, top * 2.0 ** -18)
+        step = np.where(np.abs(act) > top * 0.875 - off, np.abs(act) * 0.125, step)
+        assert np.all(np.abs(v - act) <= step + off)
+    for b in da + (wc, ws, x, y, out, oc, os_):
+        b.free()
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 896, 4864), (7, 896, 4864), (33, 416, 2080), (130, 896, 4864)])
 def test_recorded_product(fresh_lib, recorded, M, N, K):
     """Recorded ahead of any eager call, replayed with other work between: what the eager call gives, or its parts in another
@@ -600,6 +655,11 @@ def test_refusals(lib):
         (c.tlhip_rmsnorm_res_mxfp8, (p, p, 65, p, None, p, p, 32, 1e-6, 1), EUNSUPPORTED),
         (c.tlhip_rmsnorm_res_mxfp8, (p, p, -1, p, None, p, p, 32, 1e-6, 1), EUNSUPPORTED),
         (c.tlhip_rmsnorm_res_mxfp8, (p, None, 0, p, odd, p, p, 32, 1e-6, 1), EINVAL),
+        (c.tlhip_rmsnorm_res_mxfp8, (p, None, 0, p, None, p, p, 32, 1e-6, (1 << 20) + 1), EUNSUPPORTED),
+        (c.tlhip_gemm_mxfp4_nt, (p, p, p, p, p, 1 << 20, 1 << 24, 32), EUNSUPPORTED),
+        (c.tlhip_gemm_mxfp4_nt_swiglu, (p, p, p, p, p, p, 1 << 20, 1 << 20, 32), EUNSUPPORTED),
+        (c.tlhip_gemv_mxfp4_attn, (p, 1, 1, 32, p, p, p, 1, 32), EINVAL), (c.tlhip_gemv_mxfp4_attn, (p, 17, 2, 64, p, p, p, 1, 128), EUNSUPPORTED),
+        (c.tlhip_gemv_mxfp4_attn, (p, 1, 1, 64, p, p, p, 1, 64), EUNSUPPORTED), (c.tlhip_gemv_mxfp4_attn, (None, 1, 2, 64, p, p, p, 1, 128), EINVAL),
         (c.tlhip_rmsnorm_res_mxfp8, (p, None, 0, p, None, p, p, 32, 1e-6, 0), EINVAL),
         (c.tlhip_gemv_mxfp4, (p, p, p, None, 1, 32), EINVAL), (c.tlhip_gemv_mxfp4, (p, p, p, p, 1, 48), EINVAL),
         (c.tlhip_gemv_mxfp4, (p, odd, p, p, 1, 32), EINVAL), (c.tlhip_gemv_mxfp4, (p, p, p, p, 0, 32), EINVAL),
@@ -617,6 +677,15 @@ def test_refusals(lib):
         (c.tlhip_gemm_mxfp4_nt_swiglu, (p, p, p, p, p, p, 1, 33, 32), EINVAL),
         (c.tlhip_gemm_mxfp4_nt_swiglu, (p, p, p, p, p, None, 1, 32, 32), EINVAL),
         (c.tlhip_gemm_mxfp4_nt_swiglu, (p, p, p, p, odd, p, 1, 32, 32), EINVAL),
+    ]
+    q, t, u = p + 4096, p + 8192, p + 12288      # written over what is read
+    cases += [
+        (c.tlhip_quantize_mxfp4, (p, 0, p, t, 1, 32), EINVAL), (c.tlhip_quantize_mxfp4, (p, 0, q, q, 1, 32), EINVAL),
+        (c.tlhip_quantize_mxfp8, (p, p, t, 1, 32), EINVAL), (c.tlhip_quantize_mxfp8, (p, q, p, 1, 32), EINVAL),
+        (c.tlhip_dequantize_mxfp4, (p, q, p, 0, 1, 32), EINVAL), (c.tlhip_dequantize_mxfp8, (p, q, q, 0, 1, 32), EINVAL),
+        (c.tlhip_rmsnorm_res_mxfp8, (p, None, 0, q, None, p, t, 32, 1e-6, 1), EINVAL), (c.tlhip_rmsnorm_res_mxfp8, (p, None, 0, q, None, q, t, 32, 1e-6, 1), EINVAL),
+        (c.tlhip_rmsnorm_res_mxfp8, (p, q, 1, t, p, q, u, 32, 1e-6, 1), EINVAL), (c.tlhip_rmsnorm_res_mxfp8, (p, None, 0, q, p, t, p, 32, 1e-6, 1), EINVAL),
+        (c.tlhip_gemm_mxfp4_nt_swiglu, (p, q, t, u, p, u + 64, 1, 32, 32), EINVAL), (c.tlhip_gemm_mxfp4_nt_swiglu, (p, q, t, u, u + 64, q, 1, 32, 32), EINVAL),
     ]
     before = lib.census()
     for fn, args, want in cases:
