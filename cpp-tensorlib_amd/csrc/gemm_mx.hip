@@ -297,11 +297,11 @@ int tlhip_gemm_mxfp4_nt_parts(const void* acodes, const void* ascales, const voi
   if (!n_parts) return fail(TLHIP_EINVAL, "%s: null pointer", who);
   if (parts_bytes < M * N * 4) return fail(TLHIP_EINVAL, "%s: the parts need M * N * 4 bytes at least", who);
   hipError_t e;
-  if (M <= kMxFewRows) {
+  const MxPlan P = plan_tiles(M, N, K, parts_bytes / (M * N * 4), false, false);
+  if (mx_few_rows_us(M, N, K) < P.us) {
     *n_parts = 1;
     e = launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, static_cast<float*>(parts), nullptr, nullptr);
   } else {
-    const MxPlan P = plan_tiles(M, N, K, parts_bytes / (M * N * 4), false, false);
     *n_parts = P.parts;
     e = launch_plan(P, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, M * N, static_cast<float*>(parts), nullptr, nullptr);
   }
@@ -315,10 +315,10 @@ int tlhip_gemm_mxfp4_nt(const void* acodes, const void* ascales, const void* cod
   const char* who = "tlhip_gemm_mxfp4_nt";
   if (const int rc = check_mx_product(who, acodes, ascales, codes, scales, C, M, N, K)) return rc;
   hipError_t e;
-  if (M <= kMxFewRows) {
+  MxPlan P = plan_tiles(M, N, K, 16, false, true);
+  if (mx_few_rows_us(M, N, K) < P.us) {
     e = launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, static_cast<float*>(C), nullptr, nullptr);
   } else {
-    MxPlan P = plan_tiles(M, N, K, 16, false, true);
     const int64_t apart = (M * N + 3) & ~(int64_t)3;
     float* out = static_cast<float*>(C);
     if (P.parts > 1) {
@@ -348,18 +348,22 @@ int tlhip_gemm_mxfp4_nt_swiglu(const void* acodes, const void* ascales, const vo
     return fail(TLHIP_EINVAL, "%s: the activation must not be written over the rows", who);
   uint8_t *qc = static_cast<uint8_t*>(act_codes), *qs = static_cast<uint8_t*>(act_scales);
   // Few tiles over a long K: gate and up products in parts, and a launch that adds them up and gates (us so, and in one launch: 282 x 32 x 11552
-  // 12.5, 55.9; 310 x 832 x 8128 26.5, 49.9). For up to 16 rows blocks of 16 features then, not of 32 gate and 32 up rows (12 x 32 x 10368 11.5, 16.3; 7 x
-  // 1792 x 5440 9.1, 11.7; 16 x 512 x 1536 7.7, 8.1; 1024 7.6, 7.9; 16 x 6144 x 3584, where blocks of 64 rows fill the CUs, 14.0, 11.3).
+  // 12.5, 55.9; 310 x 832 x 8128 26.5, 49.9). Of few rows the products are then those of 16 rows
+  // a block, or of tiles in parts, as their estimates say; up to 16 rows the one launch has blocks of 32 gate and 32 up rows (12 x 32 x 10368
+  // 11.5, 16.3; 7 x 1792 x 5440 9.1, 11.7; 16 x 512 x 1536 7.7, 8.1; 1024 7.6, 7.9; 16 x 6144 x 3584, where those fill the CUs, 14.0, 11.3).
   const bool few = M <= kMxFewRows;
   const MxPlan one = plan_tiles(M, ff, K, 1, true, false);
-  MxPlan two = plan_tiles(M, 2 * ff, K, few ? 1 : 16, false, false);
-  if (two.parts == 1) two.us += 4.0 * (double)M * (double)ff * 4.0 / 5.4e6;
+  MxPlan two = plan_tiles(M, 2 * ff, K, 16, false, false);
+  const double rows_us = mx_few_rows_us(M, 2 * ff, K), whole = 4.0 * (double)M * (double)ff * 4.0 / 5.4e6;    // (of one part, written and read)
+  if (two.parts == 1) two.us += whole;
+  const bool rows = rows_us + whole < two.us;
+  if (rows) two = MxPlan{0, 1, rows_us + whole};
   const bool apart = few ? !mx_few_rows_fit(ff, K, true) || (K >= 1536 && ff / kMxBlock <= cu_count() / 2) : two.us + 2.2 < one.us;
   float* const parts = apart ? static_cast<float*>(scratch((size_t)two.parts * M * 2 * ff * 4)) : nullptr;    // (a recording may not grow it)
   hipError_t e;
   if (parts) {
-    e = few ? launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, 2 * ff, K, parts, nullptr, nullptr)
-            : launch_plan(two, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, 2 * ff, K, M * 2 * ff, parts, nullptr, nullptr);
+    e = rows ? launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, 2 * ff, K, parts, nullptr, nullptr)
+             : launch_plan(two, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, 2 * ff, K, M * 2 * ff, parts, nullptr, nullptr);
     if (e == hipSuccess)
       mx_gate_sum_kernel<<<dim3((unsigned)((M * (ff / 4) + 255) / 256)), dim3(256), 0, ctx().stream>>>(reinterpret_cast<const float4*>(parts), qc, qs, M,
                                                                                                        (int)(ff / 4), two.parts);

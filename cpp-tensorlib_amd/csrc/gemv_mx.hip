@@ -1,5 +1,5 @@
 // Products of few rows over MXFP4 weights: of one f32 row (a decode step's, plain or behind an RMS norm, with or without the gated
-// activation) and of up to 16 MXFP8 rows. All of it is bound by reading the weight.
+// activation) and of MXFP8 rows, 16 to a block. All of it is bound by reading the weight.
 #include "mx_mfma.hpp"
 
 #include <algorithm>
@@ -10,7 +10,7 @@ namespace tlhip {
 // of its rows and every KW-th unit of 256 k (128 bytes of a row). KW wavefronts of a block share rows; their sums are joined in
 // LDS, in their order. Features that are left over are the last row's again, and not stored.
 //
-// kCodes: up to 16 NT rows of MXFP8, read by every block, in two parts each (above).
+// kCodes: 16 rows of MXFP8 a block, in two parts each (mx_mfma.hpp).
 // kFloat, kNormed: one f32 row (kNormed: rms-normed first), cut into digits that the matrix cores multiply exactly. A number's magnitude,
 // over the power of two of its block's largest, is a whole number of 48 bits: twelve digits of four. A byte 0 to 15 is,
 // as e4m3, that many times 2^-9, so a digit is its own code; with the number's sign it is one element of a row of the second operand,
@@ -170,7 +170,8 @@ __global__ __launch_bounds__(SRC == kCodes ? 512 : 1024, 2) void mx_rows_kernel(
     wrow[f] = W + ((t.up ? (int64_t)N : 0) + min(n0 + t.n, N - 1)) * nb * 16;
     wscale[f] = (fw * kTile + t.n) * nb + (t.up ? whole_16(FW * kTile * nb) : 0);
   }
-  const uint8_t *arow = A + (int64_t)min(r, M - 1) * nb * 32, *ascale = sa + (int64_t)min(r, M - 1) * nb;
+  const int m = SRC == kCodes ? 16 * blockIdx.y + r : 0;        // my row of the activations
+  const uint8_t *arow = A + (int64_t)min(m, M - 1) * nb * 32, *ascale = sa + (int64_t)min(m, M - 1) * nb;
   struct Unit {
     frag16 w[2][NF];
     frag16 lo[2], hi[2];
@@ -328,14 +329,14 @@ __global__ __launch_bounds__(SRC == kCodes ? 512 : 1024, 2) void mx_rows_kernel(
 #pragma unroll
     for (int p = 0; p < NF / 4; p++) {
       const int n = n0 + 32 * p;
-      const int64_t m = min(r, M - 1);
-      store_gated(c[2 * p], c[2 * p + 1], c[NF / 2 + 2 * p], c[NF / 2 + 2 * p + 1], g, r < M && n < N, codes + m * N + n,
-                  scales + m * (N / kMxBlock) + n / kMxBlock);
+      const int64_t at = min(m, M - 1);
+      store_gated(c[2 * p], c[2 * p + 1], c[NF / 2 + 2 * p], c[NF / 2 + 2 * p + 1], g, m < M && n < N, codes + at * N + n,
+                  scales + at * (N / kMxBlock) + n / kMxBlock);
     }
   } else {
 #pragma unroll
     for (int f = 0; f < NF; f++)
-      if (my_tile(f) && r < M) store_features(C + (int64_t)r * N, n0 + 16 * f + 4 * g, N, c[f]);
+      if (my_tile(f) && m < M) store_features(C + (int64_t)m * N, n0 + 16 * f + 4 * g, N, c[f]);
   }
 }
 
@@ -348,7 +349,7 @@ static hipError_t launch_rows(const uint8_t* A, const uint8_t* sa, const uint8_t
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
   if (e != hipSuccess) return e;
   const int64_t per_block = (int64_t)kTile * (waves / KW);
-  kernel<<<dim3((unsigned)((N + per_block - 1) / per_block)), dim3(64 * waves), lds, ctx().stream>>>(
+  kernel<<<dim3((unsigned)((N + per_block - 1) / per_block), SRC == kCodes ? (unsigned)((M + 15) / 16) : 1u), dim3(64 * waves), lds, ctx().stream>>>(
       A, sa, W, sw, (int)M, (int)N, (int)(K / kMxBlock), KW, waves, C, codes, scales, R);
   return hipGetLastError();
 }
@@ -711,11 +712,21 @@ bool mx_few_rows_fit(int64_t N, int64_t K, bool gated) {
   // (a gated block has the scales of 64 rows in LDS beside 32 KB of sums)
   return !gated || 64 * (K / kMxBlock) <= 120 * 1024;
 }
+// 16 rows of the weight a block, 32 where there would be more blocks than CUs (77 x 896 x 4864 7.4 us, with 16 8.9)
+static int rows_tiles(int64_t M, int64_t N, int64_t K) { return (N + 15) / 16 * ((M + 15) / 16) > cu_count() && K <= 32768 ? 2 : 1; }
+// Up to a block on each CU it takes 2.9 us and 27 ns for each KB that a block reads, of both operands; up to two blocks twice that, beyond which
+// tiles that share what they read are ahead (measured 17 to 256 rows by 896 x 896 to 4608 x 3584: 48 x 896 x 4864 5.6, estimated 6.0, in
+// tiles 6.9; 112 x 1152 x 896 3.7, 3.9, 5.3; 48 x 3584 x 3584 9.7, 9.1, 9.1).
+double mx_few_rows_us(int64_t M, int64_t N, int64_t K) {
+  const int64_t nf = rows_tiles(M, N, K), blocks = (N + 16 * nf - 1) / (16 * nf) * ((M + 15) / 16), cus = cu_count();
+  if (blocks > 2 * cus) return M <= kMxFewRows ? 0 : 1e30;
+  return 2.9 + (double)((blocks + cus - 1) / cus) * (double)(nf * K * 17 / 2 + std::min<int64_t>(M, 16) * K) / 1024 * 0.027;
+}
 hipError_t launch_mx_few_rows(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N, int64_t K, float* C,
                               uint8_t* codes, uint8_t* scales) {
   if (codes) return launch_rows<kCodes, 4, true>(A, sa, W, sw, M, N, K, 8, 8, C, codes, scales, MxRow{});
-  return (N > 16 * cu_count() && K <= 32768 ? launch_rows<kCodes, 2, false> : launch_rows<kCodes, 1, false>)(A, sa, W, sw, M, N, K, 8, 8, C, nullptr,
-                                                                                                       nullptr, MxRow{});
+  return (rows_tiles(M, N, K) == 2 ? launch_rows<kCodes, 2, false> : launch_rows<kCodes, 1, false>)(A, sa, W, sw, M, N, K, 8, 8, C, nullptr, nullptr,
+                                                                                                  MxRow{});
 }
 
 }  // namespace tlhip

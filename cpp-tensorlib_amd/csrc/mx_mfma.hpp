@@ -36,8 +36,10 @@ inline int check_mx_product(const char* who, const void* a, const void* sa, cons
   return TLHIP_OK;
 }
 
-// gemv_mx.hip: up to kMxFewRows rows of MXFP8 by a weight; codes non-null: gated, [gate | up] rows of N each, into MXFP8.
+// gemv_mx.hip: rows of MXFP8 by a weight, 16 of them a block; codes non-null: gated, [gate | up] rows of N each, into MXFP8 (up to
+// kMxFewRows rows). mx_few_rows_us: what it takes without the gate, nothing where no other kernel reads the weight as fast.
 constexpr int kMxFewRows = 16;
+double mx_few_rows_us(int64_t M, int64_t N, int64_t K);
 bool mx_few_rows_fit(int64_t N, int64_t K, bool gated);
 hipError_t launch_mx_few_rows(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N, int64_t K, float* C,
                               uint8_t* codes, uint8_t* scales);
