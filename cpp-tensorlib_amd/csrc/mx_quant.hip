@@ -133,11 +133,12 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
 // which stay in its registers. The statistic and h are formed in 64 bits and h is rounded to f32 once: an element next to the border
 // between two codes then falls on the same side however the sum is split, so a row's bytes do not depend on the launch's shape.
 // One row of 896 4.4 us (with the row in LDS and the sum through shuffles 5.1; an empty launch is 3.3), 301 of 3584 with three parts
-// 7.3 (a copy's rate would be 4.2 beside the launch), 2048 of 8192 with two 59, 4.9 TB/s.
+// 7.1 (a copy's rate would be 4.2 beside the launch), 2048 of 8192 with two 58, 5.0 TB/s. Sixteen numbers a thread where eight would do: 301 of 3584
+// with three parts 6.0 instead of 6.4 in a queue of launches, but 257 with two 4.8 instead of 4.5, 2048 of 8192 60 instead of 58.
 template <int V>
 __global__ __launch_bounds__(1024) void rmsnorm_mxfp8_kernel(const float* x, const float* __restrict__ parts, int S, const float* __restrict__ w,
                                                              float* xout, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int n,
-                                                             double eps) {
+                                                             double eps, double each) {
   __shared__ double red[16];
   const int64_t r = blockIdx.x, all = (int64_t)gridDim.x * n, row = r * n;
   const int tid = threadIdx.x, threads = blockDim.x;
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(1024) void rmsnorm_mxfp8_kernel(const float* x, con
     ss = 0;
     for (int k = 0; k < threads / 64; k++) ss += red[k];
   }
-  const double inv = rsqrt(ss / n + eps);
+  const double inv = rsqrt(ss * each + eps);       // (each: 1 / n)
 #pragma unroll
   for (int k = 0; k < V; k++) {
     const int i = 8 * (tid + k * threads);
@@ -286,7 +287,7 @@ int tlhip_rmsnorm_res_mxfp8(const void* x, const void* parts, int64_t S, const v
   const auto kernel = V == 1 ? rmsnorm_mxfp8_kernel<1> : V == 2 ? rmsnorm_mxfp8_kernel<2> : rmsnorm_mxfp8_kernel<4>;
   kernel<<<dim3((unsigned)rows), dim3((unsigned)threads), 0, ctx().stream>>>(
       static_cast<const float*>(x), static_cast<const float*>(parts), (int)S, static_cast<const float*>(w), static_cast<float*>(xout),
-      static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), (int)n, (double)eps);
+      static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), (int)n, (double)eps, 1.0 / (double)n);
   TLHIP_CHECK_LAUNCH(TLHIP_C_RMSNORM_RES);
 }
 
