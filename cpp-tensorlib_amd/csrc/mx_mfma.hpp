@@ -91,8 +91,10 @@ __device__ __forceinline__ void store_gated(const v4f& g0, const v4f& g1, const 
     v[4 + k] = gated_fast(g1[k], u1[k]);
     big = max(big, max(magnitude(v[k]), magnitude(v[4 + k])));
   }
-  big = max(big, (uint32_t)__shfl_xor((int)big, 16, kWave));
-  big = max(big, (uint32_t)__shfl_xor((int)big, 32, kWave));
+  const auto by16 = __builtin_amdgcn_permlane16_swap(big, big, false, false);      // with the lane 16 away, then 32
+  big = max(by16[0], by16[1]);
+  const auto by32 = __builtin_amdgcn_permlane32_swap(big, big, false, false);
+  big = max(by32[0], by32[1]);
   const uint32_t s = mx_scale_of(big, kMx8Exp);
   const float up = mx_up(min(s, 252u));
 #pragma unroll
