@@ -18,15 +18,11 @@ namespace tlhip {
 // 422 us (1.32e15 a second), 512 x 3584 x 18944 66 us (1.05e15, four parts' traffic and their sum in it). The activations straight
 // into registers took 484 us instead of 436; a third stage of LDS and raised wave priorities changed nothing.
 typedef uint32_t any4 __attribute__((aligned(1)));
-__device__ __forceinline__ uint32_t four_scales(const uint8_t* row, int b, int nb) {      // bytes b .. b + 3 of nb, 0 past them (b < nb)
-  if (nb < 4) {
-    uint32_t v = row[0];
-    if (nb > 1) v |= (uint32_t)row[1] << 8;
-    if (nb > 2) v |= (uint32_t)row[2] << 16;
-    return v;
-  }
-  const int at = min(b, nb - 4);
-  return *reinterpret_cast<const any4*>(row + at) >> (8 * (b - at));
+__device__ __forceinline__ uint32_t short_row(const uint8_t* row, int nb) {      // the scales of a row that has one to three
+  uint32_t v = row[0];
+  if (nb > 1) v |= (uint32_t)row[1] << 8;
+  if (nb > 2) v |= (uint32_t)row[2] << 16;
+  return v;
 }
 struct MxTiles {
   int tokens, count;       // tiles of tokens, all tiles
@@ -60,16 +56,17 @@ __global__ __launch_bounds__(64 * WF * WT, WPE) void mx_tile_kernel(const uint8_
 
   // Rows of a wavefront's copies, 16 of the weight or 8 of the activations: the first one's address (uniform) and 32-bit offsets
   const uint8_t* src[kCopies];
-  uint32_t off[kCopies], chunk[kCopies];
+  uint32_t off[kCopies];
 #pragma unroll
   for (int j = 0; j < kCopies; j++) {
     const bool w = j * kWaves * 1024 < kWBytes;
     const int q = j * kWaves + wave - (w ? 0 : kWBytes / 1024), row0 = q * (w ? 16 : 8), row = row0 + (lane >> (w ? 2 : 3));
     const int64_t base = w ? weight_row(row0) : token_row(row0), mine = w ? weight_row(row) : token_row(row);
     src[j] = w ? W + base * nb * 16 : A + base * nb * 32;
-    chunk[j] = (w ? (lane & 3) ^ (-(row >> 2) & 3) : (lane & 7) ^ (row >> 1 & 7)) * 16;
     off[j] = (uint32_t)(mine - base) * (uint32_t)nb * (w ? 16u : 32u);
   }
+  // the chunk of its row that a lane copies: W's lanes & 3 ^ (-(row >> 2) & 3), A's lane & 7 ^ (row >> 1 & 7), rows of a copy being whole 16s and 8s
+  const uint32_t wchunk = ((lane & 3) ^ (-(lane >> 4) & 3)) * 16, achunk = ((lane & 7) ^ (lane >> 4)) * 16;
   const uint8_t* srow[kRowsEach];
   uint32_t sc[kRowsEach];
 #pragma unroll
@@ -77,16 +74,22 @@ __global__ __launch_bounds__(64 * WF * WT, WPE) void mx_tile_kernel(const uint8_
     const int i = min(j * kThreads + tid, kRows - 1);
     srow[j] = i < TF ? sw + weight_row(i) * nb : sa + token_row(i - TF) * nb;
   }
+  // Scale words that are not whole ones go through registers, two steps ahead, so that nobody waits for them (301 x 4608 x 3648 18.9 us,
+  // 26.7 where each step waited; x 3712, whose are words, 17.4)
+  const auto ask_scales = [&](int step) {
+    if constexpr (!WORDS) {
+      if (nb >= 4) {
+#pragma unroll
+        for (int j = 0; j < kRowsEach; j++) sc[j] = *reinterpret_cast<const any4*>(srow[j] + min((first + step) * 4, nb - 4));
+      }
+    }
+  };
   const auto copy = [&](int step, int stage) {
     char* s = lds + stage * kStage;
-    if constexpr (!WORDS) {
-#pragma unroll
-      for (int j = 0; j < kRowsEach; j++) sc[j] = four_scales(srow[j], (first + step) * 4, nb);
-    }
 #pragma unroll
     for (int j = 0; j < kCopies; j++) {
       const bool w = j * kWaves * 1024 < kWBytes;
-      uint32_t k = (uint32_t)(first + step) * (w ? 64u : 128u) + chunk[j];
+      uint32_t k = (uint32_t)(first + step) * (w ? 64u : 128u) + (w ? wchunk : achunk ^ (uint32_t)((j * kWaves + wave - kWBytes / 1024) & 1) * 64u);
       if constexpr (!WORDS) k = min(k, (uint32_t)(w ? nb - 1 : 2 * nb - 1) * 16u);
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[j] + (off[j] + k)),
                                        (__attribute__((address_space(3))) void*)(s + (j * kWaves + wave) * 1024), 16, 0, 0);
@@ -99,11 +102,12 @@ __global__ __launch_bounds__(64 * WF * WT, WPE) void mx_tile_kernel(const uint8_
                                            (__attribute__((address_space(3))) void*)(s + kElems + (j * kThreads + wave * 64) * 4), 4, 0, 0);
     }
   };
-  const auto keep_scales = [&](int stage) {      // of the step copied last
+  const auto keep_scales = [&](int step, int stage) {      // those asked for last; a row's last word has been read from before its end
     if constexpr (!WORDS) {
+      const int past = nb < 4 ? 0 : 8 * max((first + step) * 4 - (nb - 4), 0);
 #pragma unroll
       for (int j = 0; j < kRowsEach; j++)
-        if (j * kThreads + tid < kRows) *reinterpret_cast<uint32_t*>(lds + stage * kStage + kElems + (j * kThreads + tid) * 4) = sc[j];
+        if (j * kThreads + tid < kRows) *reinterpret_cast<uint32_t*>(lds + stage * kStage + kElems + (j * kThreads + tid) * 4) = sc[j] >> past;
     }
   };
 
@@ -118,14 +122,26 @@ __global__ __launch_bounds__(64 * WF * WT, WPE) void mx_tile_kernel(const uint8_
   const int a0 = arow + ((g ^ ax) << 4), a1 = arow + (((4 + g) ^ ax) << 4);
   const int ws = kElems + (wf * 16 * NF + r) * 4, as = kElems + (TF + wt * 16 * NT + r) * 4;   // (+ 64 a tile)
 
+  if constexpr (!WORDS) {
+    if (nb < 4) {                                // (one step)
+#pragma unroll
+      for (int j = 0; j < kRowsEach; j++) sc[j] = short_row(srow[j], nb);
+    }
+  }
+  ask_scales(0);
   copy(0, 0);
-  keep_scales(0);
+  keep_scales(0, 0);
+  ask_scales(1);
   for (int i = 0; i < steps; i++) {
     // what was copied a step ago has landed, my reads are done, and so are everybody's
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (i + 1 < steps) copy(i + 1, (i + 1) & 1);
+    if (i + 1 < steps) {
+      keep_scales(i + 1, (i + 1) & 1);
+      ask_scales(i + 2);
+      copy(i + 1, (i + 1) & 1);
+    }
     // LDS is read as vectors of words, never as uint4, which the compiler takes for something that a copy in flight may write
     const char* s = lds + (i & 1) * kStage;
     frag16 w[NF];
@@ -148,7 +164,6 @@ __global__ __launch_bounds__(64 * WF * WT, WPE) void mx_tile_kernel(const uint8_
       for (int f = 0; f < NF; f++)
         c[f][t] = mx_mma(weight_operand(w[f]), large, c[f][t], swv[f], sav);
     }
-    if (i + 1 < steps) keep_scales((i + 1) & 1);
   }
 #pragma unroll
   for (int f = 0; f < NF; f++)

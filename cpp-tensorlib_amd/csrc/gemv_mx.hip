@@ -724,8 +724,10 @@ double mx_few_rows_us(int64_t M, int64_t N, int64_t K) {
 }
 hipError_t launch_mx_few_rows(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N, int64_t K, float* C,
                               uint8_t* codes, uint8_t* scales) {
-  if (codes) return launch_rows<kCodes, 4, true>(A, sa, W, sw, M, N, K, 8, 8, C, codes, scales, MxRow{});
-  return (rows_tiles(M, N, K) == 2 ? launch_rows<kCodes, 2, false> : launch_rows<kCodes, 1, false>)(A, sa, W, sw, M, N, K, 8, 8, C, nullptr, nullptr,
+  const int64_t units = (K + 255) / 256;
+  const int KW = units <= 1 ? 1 : units <= 2 ? 2 : units <= 4 ? 4 : 8;
+  if (codes) return launch_rows<kCodes, 4, true>(A, sa, W, sw, M, N, K, KW, KW, C, codes, scales, MxRow{});
+  return (rows_tiles(M, N, K) == 2 ? launch_rows<kCodes, 2, false> : launch_rows<kCodes, 1, false>)(A, sa, W, sw, M, N, K, KW, KW, C, nullptr, nullptr,
                                                                                                   MxRow{});
 }
 
