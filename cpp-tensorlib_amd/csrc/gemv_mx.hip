@@ -674,7 +674,8 @@ static hipError_t launch_row_small(const uint8_t* W, const uint8_t* sw, int64_t 
 }
 
 // Which kernel, by sizes (us so, and in the other forms; weights not in any cache; "gated" and "normed" as told, else plain):
-//   up to 20 2^20 elements (behind a producer 9 2^20, or 1024 rows, of up to 32768), K from 512: mx_row_small_kernel, a wavefront for every 1024 k
+//   up to 20 2^20 elements (behind a producer 9 2^20) or 1024 rows (of up to 32768 behind a producer), K from 512, from 896 where there are more
+//     than 16384 rows (30000 x 640 5.6, 5.1 in mx_row_tiles_kernel; 20000 x 1024 4.8, 5.6): mx_row_small_kernel, a wavefront for every 1024 k
 //     (896 x 4864 3.9, mx_rows_kernel 4.4; 3584 x 3584 4.1, 4.6; 1000 x 18944 5.2, 9.2; beyond, 8192 x 3584 6.0, 5.7. Normed 896 x 4864 4.3,
 //     5.1; 9728 x 896 4.3, 4.5, gated 4.4, 4.8; 1000 x 18944 8.6, 12.0; beyond, 3584 x 3584 5.6, 5.1; 20000 x 512 5.0, 4.5). Four rows a
 //     wavefront (1000 x 18944 5.2, two 6.2; 3584 x 3584 4.1, 4.4), two where that makes no more blocks than there are CUs (normed
@@ -693,7 +694,8 @@ static hipError_t launch_row(const uint8_t* W, const uint8_t* sw, int64_t N, int
   const int64_t rows = (GATED ? 8 : 16) * (8 / KW);          // of a tile, gate rows if gated
   const int64_t all = GATED ? 2 * N : N;                     // rows of the weight
   if constexpr (SRC == kFloat) {
-    if (all * K <= (int64_t)20 << 20 && K >= 512) return launch_row_small<SRC, 4, false>(W, sw, N, K, (int)std::min<int64_t>(16, (K + 1023) / 1024), 1, y, R);
+    if ((all * K <= (int64_t)20 << 20 || all <= 4 * cus) && K >= 512 && (K >= 896 || all <= 64 * cus))
+      return launch_row_small<SRC, 4, false>(W, sw, N, K, (int)std::min<int64_t>(16, (K + 1023) / 1024), 1, y, R);
   } else {
     if ((all * K <= (int64_t)9 << 20 || all <= 4 * cus) && K >= 512 && K <= 32768) {
       const int kw = (int)std::min<int64_t>(16, (K + 1023) / 1024), fw = kw <= 8 ? 2 : 1;
