@@ -15,7 +15,7 @@ namespace tlhip {
 // from wherever it lies.
 // Bound by the matrix cores: each element is multiplied twice, as its large and its small half, so their ceiling is half the
 // formats' (about 1.9e15 products and sums a second at the clock that such a load leaves). 2048 x 37888 x 3584 with the gate takes
-// 422 us (1.32e15 a second), 512 x 3584 x 18944 66 us (1.05e15, four parts' traffic and their sum in it). The activations straight
+// 390 us (1.43e15 a second), 512 x 3584 x 18944 66 us (1.05e15, four parts' traffic and their sum in it). The activations straight
 // into registers took 484 us instead of 436; a third stage of LDS and raised wave priorities changed nothing.
 typedef uint32_t any4 __attribute__((aligned(1)));
 __device__ __forceinline__ uint32_t short_row(const uint8_t* row, int nb) {      // the scales of a row that has one to three
@@ -218,7 +218,7 @@ static hipError_t launch_tiles(const uint8_t* A, const uint8_t* sa, const uint8_
 // Features x tokens of a tile. A step takes `one` us plus `more` for each block on a CU, as measured on products of 20 to 2048 rows by 896 x 4864
 // to 37888 x 3584; the launch that adds parts up 2.2 us and their traffic at 5.4 TB/s. Over 54 products of those sizes the choice takes 1.01
 // times the best one's time in the mean and 1.16 at worst. Both sides: 77 x 896 x 4864 7.6 us in 8 parts of 64 x 64, 8.7 of 128 x 64, 23.9 in
-// one; 512 x 18944 gated x 3584 116 us with 128 x 128, 132 with 256 x 128, 137 with 128 x 64, 162 with 64 x 64; 2048 so 422 with 256 x 128, 427
+// one; with the result read back (5 us of it) 512 x 18944 gated x 3584 116 us with 128 x 128, 132 with 256 x 128, 137 with 128 x 64, 162 with 64 x 64; 2048 x 37888 x 3584 422 with 256 x 128, 427
 // with 128 x 128, 532 with 128 x 64. Numbers of parts that the eight dies do not share evenly are not tried (77 x 3584 x 18944 in 10
 // parts 30.4 us, in 8 23.5, in 12 26.2).
 struct MxPlan { int variant = 0, parts = 1; double us = 1e30; };
@@ -362,7 +362,8 @@ int tlhip_gemm_mxfp4_nt_swiglu(const void* acodes, const void* ascales, const vo
   if (act_codes == acodes || act_scales == ascales || act_codes == act_scales)
     return fail(TLHIP_EINVAL, "%s: the activation must not be written over the rows", who);
   uint8_t *qc = static_cast<uint8_t*>(act_codes), *qs = static_cast<uint8_t*>(act_scales);
-  // Few tiles over a long K: gate and up products in parts, and a launch that adds them up and gates (us so, and in one launch: 282 x 32 x 11552
+  // Few tiles over a long K: gate and up products in parts, and a launch that adds them up and gates (us so, and in one launch, each with the
+  // result read back, 2 to 3 of them: 282 x 32 x 11552
   // 12.5, 55.9; 310 x 832 x 8128 26.5, 49.9). Of few rows the products are then those of 16 rows
   // a block, or of tiles in parts, as their estimates say; up to 16 rows the one launch has blocks of 32 gate and 32 up rows (12 x 32 x 10368
   // 11.5, 16.3; 7 x 1792 x 5440 9.1, 11.7; 16 x 512 x 1536 7.7, 8.1; 1024 7.6, 7.9; 16 x 6144 x 3584, where those fill the CUs, 14.0, 11.3).

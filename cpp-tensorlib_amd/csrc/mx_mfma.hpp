@@ -72,7 +72,8 @@ __device__ __forceinline__ v8i row_operand(const frag16& lo, const frag16& hi) {
 // What gemv_shared.hpp's gated() is, on the hardware's exponential and reciprocal (1 ulp each): e^-g = 2^t, t = -g log2 e in two terms, the
 // lower one as the first two of its series; from t = 128 on 0. The reciprocal knows no subnormal numbers: it is of (1 + e^-g) / 4.
 // As far from 64 bits as the exact operations are (4.7e-8 in the mean over gates of order one, 2.6e-7 at most; those 4.7e-8, 2.8e-7), in
-// thirteen instructions instead of more than thirty: 1280 x 4160 gated x 96 15.0 us instead of 17.4, 2048 x 18944 x 3584 422 instead of 431.
+// thirteen instructions instead of more than thirty: 1280 x 4160 gated x 96 15.0 us instead of 17.4, 2048 x 18944 x 3584 422 instead
+// of 431 (with the results read back, 3.7 and 18 of them).
 __device__ __forceinline__ float gated_fast(float g, float u) {
   const float t = g * -1.44269502f, r = fmaf(g, -1.92596299e-8f, fmaf(g, -1.44269502f, -t));
   float e = __builtin_amdgcn_exp2f(t);
