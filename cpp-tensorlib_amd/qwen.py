@@ -369,7 +369,7 @@ class QwenGPU:
         self.L.tlq_set_merge_in_oproj(self.h, 1 if on else 0)
 
     def set_fused_prefill(self, on):
-        """Prompt chunks: one launch for split_heads + rope + kv_fill and token-major attention output (default), or the reference's op sequence."""
+        """Prompt chunks: one launch for split_heads + rope + kv_fill and token-major attention output (default; always over MXFP4 weights), or the reference's op sequence."""
         self.L.tlq_set_fused_prefill(self.h, 1 if on else 0)
 
     def set_prompt_f16(self, on):
@@ -377,7 +377,7 @@ class QwenGPU:
         self.L.tlq_set_prompt_f16(self.h, 1 if on else 0)
 
     def set_gateup_epilogue(self, on):
-        """Within the fused path: swiglu as the epilogue of the gate|up GEMV (default) or as the producer of the down GEMV."""
+        """Within the fused path: swiglu as the epilogue of the gate|up GEMV (default; always over MXFP4 weights) or as the producer of the down GEMV."""
         self.L.tlq_set_gateup_epilogue(self.h, 1 if on else 0)
 
     def flush(self):

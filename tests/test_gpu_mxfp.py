@@ -621,6 +621,33 @@ def test_recorded_layer(fresh_lib, recorded):
     assert np.array_equal(replays[0], replays[1]) and np.array_equal(replays[0], replays[2])
 
 
+@pytest.mark.parametrize("M,N,K", [(40, 192, 8192), (20, 576, 9408), (9, 192, 8224)])
+def test_recorded_products_in_parts(fresh_lib, recorded, M, N, K):
+    """Behind an eager call, so that there is a workspace: products of few tiles in parts, plain and gated, replayed with other work on
+    the same workspace between: the eager call's bytes."""
+    lib, r = fresh_lib, rng(91, M, K)
+    da, dw = upload_rows(lib, *rows8(r, M, K)), upload_rows(lib, *weight(r, N, K), True)
+    other = upload_rows(lib, *rows8(r, 60, K))
+    y, ff = lib.empty((M, N)), N // 2
+    codes, scales, dump = lib.empty_bytes(M * ff), lib.empty_bytes(M * ff // 32), lib.empty((60, N))
+    both = lib.empty_bytes(M * N * 4 + M * ff + M * ff // 32)
+
+    def calls():
+        lib.gemm_mxfp4_nt(*da, *dw, y, M, N, K)
+        lib.gemm_mxfp4_nt_swiglu(*da, *dw, codes, scales, M, ff, K)
+        lib.gemm_mxfp4_nt(*other, *dw, dump, 60, N, K)
+        at = both.ptr
+        for b, n in ((y, M * N * 4), (codes, M * ff), (scales, M * ff // 32)):
+            lib._chk(lib.c.tlhip_memcpy_d2d_async(at, b.ptr, n))
+            at += n
+
+    calls()
+    lib.sync()
+    eager = both.numpy().copy()
+    for got in recorded(calls, both):
+        assert np.array_equal(got, eager)
+
+
 def test_products_are_deterministic(lib):
     r = rng(14)
     for M, N, K in [(1, 4608, 3584), (7, 896, 4864), (129, 896, 4864)]:
