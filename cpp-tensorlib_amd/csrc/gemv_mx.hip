@@ -681,7 +681,8 @@ static hipError_t launch_row_small(const uint8_t* W, const uint8_t* sw, int64_t 
 //     wavefront (1000 x 18944 5.2, two 6.2; 3584 x 3584 4.1, 4.4), two where that makes no more blocks than there are CUs (normed
 //     896 x 4864 4.3, four 4.5); two sets of wavefronts a block share what is staged.
 //   more than 4 tiles of 16 rows for each CU, K up to 4096: mx_row_tiles_kernel (152064 x 3584 51.6, row by row 55.2; 37888 x 3584 14.8, 16.0;
-//     9728 x 896, 2.4 tiles: 4.2, 4.2);
+//     9728 x 896, 2.4 tiles: 4.2, 4.2; 16384 x 2048 6.4, 6.1); more than 2 from twelve units of 256 k on, where row by row is a block of
+//     sixteen wavefronts a CU (12288 x 3584 7.6, 8.8, normed 8.6, 11.0; 8192 x 3584, 2 tiles: 6.6, 5.7);
 //   K up to 1024: as many wavefronts share a row's K as it has units of 256, in several sets (9728 x 896 in two of four 4.2, in eight 4.4;
 //     150000 x 64 in eight of one 4.8, in two of four 11.4);
 //   up to twelve units of 256 k: eight; beyond: sixteen (3584 x 18944 9.8; eight 10.8; 4608 x 3584 4.8; 5.2);
@@ -703,7 +704,7 @@ static hipError_t launch_row(const uint8_t* W, const uint8_t* sw, int64_t N, int
     }
   }
   if constexpr (SRC != kMerged)
-    if (units <= 16 && N % 16 == 0 && N > 4 * cus * rows && rows * nb % 16 == 0)
+    if (units <= 16 && N % 16 == 0 && N > (units > 12 ? 2 : 4) * cus * rows && rows * nb % 16 == 0)
       return (units <= KW ? launch_row_tiles<SRC, 1, GATED, 1> : launch_row_tiles<SRC, 1, GATED, 2>)(W, sw, N, K, KW, 2, y, R);
   const int waves = units <= 12 ? 8 : 16, kw = units <= 8 ? KW : waves;
   const bool two = (GATED ? 2 : 1) * N > 16 * cus && nb <= 1024;
