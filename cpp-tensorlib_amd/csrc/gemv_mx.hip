@@ -685,7 +685,8 @@ static hipError_t launch_row_small(const uint8_t* W, const uint8_t* sw, int64_t 
 //     sixteen wavefronts a CU (12288 x 3584 7.6, 8.8, normed 8.6, 11.0; 8192 x 3584, 2 tiles: 6.6, 5.7);
 //   K up to 1024: as many wavefronts share a row's K as it has units of 256, in several sets (9728 x 896 in two of four 4.2, in eight 4.4;
 //     150000 x 64 in eight of one 4.8, in two of four 11.4);
-//   up to twelve units of 256 k: eight; beyond: sixteen (3584 x 18944 9.8; eight 10.8; 4608 x 3584 4.8; 5.2);
+//   up to twelve units of 256 k: eight; beyond: sixteen (3584 x 18944 9.8; eight 10.8; 4608 x 3584 4.8; 5.2), but eight where there are more blocks
+//     than CUs, which hold one of sixteen (16384 x 8192 17.2, 19.5; 28672 x 8192 normed 30.4, 38.5; 32768 x 5120 gated 21.5, 30.1);
 //   32 rows a block where there are more tiles of 16 than CUs (4608 x 3584 5.1, 16: 5.9; gated 6.6, 8.8; 3584 x 18944 12.9, 16: 9.8), and while
 //     the scales of their rows leave room in LDS.
 template <int SRC, bool GATED>
@@ -706,8 +707,8 @@ static hipError_t launch_row(const uint8_t* W, const uint8_t* sw, int64_t N, int
   if constexpr (SRC != kMerged)
     if (units <= 16 && N % 16 == 0 && N > (units > 12 ? 2 : 4) * cus * rows && rows * nb % 16 == 0)
       return (units <= KW ? launch_row_tiles<SRC, 1, GATED, 1> : launch_row_tiles<SRC, 1, GATED, 2>)(W, sw, N, K, KW, 2, y, R);
-  const int waves = units <= 12 ? 8 : 16, kw = units <= 8 ? KW : waves;
-  const bool two = (GATED ? 2 : 1) * N > 16 * cus && nb <= 1024;
+  const bool two = all > 16 * cus && nb <= 1024;
+  const int waves = units <= 12 || all > (two ? 32 : 16) * cus ? 8 : 16, kw = units <= 8 ? KW : waves;
   return (two ? launch_rows<SRC, 2, GATED> : launch_rows<SRC, 1, GATED>)(nullptr, nullptr, W, sw, 1, N, K, kw, waves, y, nullptr, nullptr, R);
 }
 
