@@ -207,8 +207,7 @@ static hipError_t launch_tiles(const uint8_t* A, const uint8_t* sa, const uint8_
   const int nb = (int)(K / kMxBlock);
   const bool words = nb % 4 == 0 && ((reinterpret_cast<uintptr_t>(sa) | reinterpret_cast<uintptr_t>(sw)) & 3) == 0;
   const auto kernel = words ? mx_tile_kernel<WF, WT, NF, NT, WPE, GATED, true> : mx_tile_kernel<WF, WT, NF, NT, WPE, GATED, false>;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (e != hipSuccess) return e;
+  if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds); e != hipSuccess) return e;
   kernel<<<dim3((unsigned)P.count, (unsigned)P.parts), dim3(64 * WF * WT), lds, ctx().stream>>>(A, sa, W, sw, (int)M, (int)N, nb, P, C, codes,
                                                                                                 scales);
   return hipGetLastError();

@@ -346,8 +346,7 @@ static hipError_t launch_rows(const uint8_t* A, const uint8_t* sa, const uint8_t
   constexpr int kTile = GATED ? 8 * NF : 16 * NF;
   const int lds = std::max(SRC == kCodes ? 0 : waves * kUnitLds, rows_sums(NF, waves)) + (GATED ? 2 : 1) * whole_16((int)(waves / KW * kTile * (K / kMxBlock)));
   const auto kernel = mx_rows_kernel<SRC, NF, GATED>;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-  if (e != hipSuccess) return e;
+  if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds); e != hipSuccess) return e;
   const int64_t per_block = (int64_t)kTile * (waves / KW);
   kernel<<<dim3((unsigned)((N + per_block - 1) / per_block), SRC == kCodes ? (unsigned)((M + 15) / 16) : 1u), dim3(64 * waves), lds, ctx().stream>>>(
       A, sa, W, sw, (int)M, (int)N, (int)(K / kMxBlock), KW, waves, C, codes, scales, R);
@@ -523,8 +522,7 @@ static hipError_t launch_row_tiles(const uint8_t* W, const uint8_t* sw, int64_t 
   const int nb = (int)(K / kMxBlock), rows = 8 / KW * kTile, run = rows * nb, lds = 8 * UPW * kUnitLds + 2 * (((GATED ? 2 : 1) * run + 15) & ~15) + (2 * 8 * NF * 16 + 8) * 4;
   const int tiles = (int)((N + rows - 1) / rows);
   const auto kernel = mx_row_tiles_kernel<SRC, NF, GATED, UPW>;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-  if (e != hipSuccess) return e;
+  if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds); e != hipSuccess) return e;
   kernel<<<dim3((unsigned)std::min(tiles, per_cu * cu_count())), dim3(512), lds, ctx().stream>>>(W, sw, (int)N, nb, KW, tiles, y, R);
   return hipGetLastError();
 }
@@ -667,8 +665,7 @@ static hipError_t launch_row_small(const uint8_t* W, const uint8_t* sw, int64_t 
   const int64_t rows = FW * (GATED ? RW / 2 : RW);
   const int lds = SRC != kFloat ? (int)(K / 4 + K / 64 + 1) * 16 : 0;
   const auto kernel = mx_row_small_kernel<SRC, RW, GATED>;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 144 * 1024);
-  if (e != hipSuccess) return e;
+  if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds); e != hipSuccess) return e;
   kernel<<<dim3((unsigned)((N + rows - 1) / rows)), dim3(64 * KW * FW), lds, ctx().stream>>>(W, sw, (int)N, (int)(K / kMxBlock), KW, FW, y, R);
   return hipGetLastError();
 }

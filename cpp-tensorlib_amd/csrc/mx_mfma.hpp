@@ -36,6 +36,11 @@ inline int check_mx_product(const char* who, const void* a, const void* sa, cons
   return TLHIP_OK;
 }
 
+// More than 64 KB of LDS a block (some of it static) has to be asked for
+inline hipError_t allow_lds(const void* kernel, int lds) {
+  return lds > 60 * 1024 ? hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) : hipSuccess;
+}
+
 // gemv_mx.hip: rows of MXFP8 by a weight, 16 of them a block; codes non-null: gated, [gate | up] rows of N each, into MXFP8 (up to
 // kMxFewRows rows). mx_few_rows_us: what it takes without the gate, nothing where no other kernel reads the weight as fast.
 constexpr int kMxFewRows = 16;
