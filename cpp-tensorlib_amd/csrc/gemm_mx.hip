@@ -308,6 +308,7 @@ int tlhip_gemm_mxfp4_nt_parts(const void* acodes, const void* ascales, const voi
   TLHIP_REQUIRE_READY();
   const char* who = "tlhip_gemm_mxfp4_nt_parts";
   if (const int rc = check_mx_product(who, acodes, ascales, codes, scales, parts, M, N, K)) return rc;
+  if (const int rc = check_mx_apart(who, parts, {acodes, ascales, codes, scales})) return rc;
   if (!n_parts) return fail(TLHIP_EINVAL, "%s: null pointer", who);
   if (parts_bytes < M * N * 4) return fail(TLHIP_EINVAL, "%s: the parts need M * N * 4 bytes at least", who);
   hipError_t e;
@@ -328,6 +329,7 @@ int tlhip_gemm_mxfp4_nt(const void* acodes, const void* ascales, const void* cod
   TLHIP_REQUIRE_READY();
   const char* who = "tlhip_gemm_mxfp4_nt";
   if (const int rc = check_mx_product(who, acodes, ascales, codes, scales, C, M, N, K)) return rc;
+  if (const int rc = check_mx_apart(who, C, {acodes, ascales, codes, scales})) return rc;
   hipError_t e;
   MxPlan P = plan_tiles(M, N, K, 16, false, true);
   if (mx_few_rows_us(M, N, K) < P.us) {
@@ -358,8 +360,8 @@ int tlhip_gemm_mxfp4_nt_swiglu(const void* acodes, const void* ascales, const vo
   if (const int rc = check_mx_product(who, acodes, ascales, codes, scales, act_codes, M, ff, K)) return rc;
   if (!act_scales) return fail(TLHIP_EINVAL, "%s: null pointer", who);
   if (!mx_row(ff)) return fail(TLHIP_EINVAL, "%s: ff must be a multiple of 32", who);
-  if (act_codes == acodes || act_scales == ascales || act_codes == act_scales)
-    return fail(TLHIP_EINVAL, "%s: the activation must not be written over the rows", who);
+  if (const int rc = check_mx_apart(who, act_codes, {acodes, ascales, codes, scales, act_scales})) return rc;
+  if (const int rc = check_mx_apart(who, act_scales, {acodes, ascales, codes, scales})) return rc;
   uint8_t *qc = static_cast<uint8_t*>(act_codes), *qs = static_cast<uint8_t*>(act_scales);
   // Few tiles over a long K: gate and up products in parts, and a launch that adds them up and gates (us so, and in one launch, each with the
   // result read back, 2 to 3 of them: 282 x 32 x 11552

@@ -744,6 +744,7 @@ int tlhip_gemv_mxfp4(const void* a, const void* codes, const void* scales, void*
   TLHIP_REQUIRE_READY();
   const char* who = "tlhip_gemv_mxfp4";
   if (const int rc = check_mx_product(who, a, scales, codes, scales, y, 1, N, K)) return rc;
+  if (const int rc = check_mx_apart(who, y, {a, codes, scales})) return rc;
   const MxRow R{static_cast<const float*>(a), nullptr, nullptr, nullptr, 0.f, 0, 0, 0};
   const hipError_t e = launch_row<kFloat, false>(bytes(codes), bytes(scales), N, K, static_cast<float*>(y), R);
   if (e != hipSuccess) return hip_fail(e, who);
@@ -756,6 +757,7 @@ int tlhip_gemv_mxfp4_attn(const void* parts, int64_t n_parts, int64_t heads, int
   const char* who = "tlhip_gemv_mxfp4_attn";
   if (const int rc = check_mx_product(who, parts, scales, codes, scales, y, 1, N, K)) return rc;
   if (const int rc = check_attn_merge(parts, n_parts, heads, head_dim, K, who)) return rc;
+  if (const int rc = check_mx_apart(who, y, {parts, codes, scales})) return rc;
   const MxRow R{static_cast<const float*>(parts), nullptr, nullptr, nullptr, 0.f, (int)n_parts, (int)heads, (int)head_dim};
   const hipError_t e = launch_row<kMerged, false>(bytes(codes), bytes(scales), N, K, static_cast<float*>(y), R);
   if (e != hipSuccess) return hip_fail(e, who);
@@ -768,6 +770,9 @@ static int normed(const char* who, const void* x, const void* delta, const void*
   if (!norm_w) return fail(TLHIP_EINVAL, "%s: null pointer", who);
   if (!aligned16(delta) || !aligned16(norm_w) || !aligned16(xout)) return fail(TLHIP_EINVAL, "%s: delta, norm_w and xout must be 16-byte aligned", who);
   if (xout && (xout == x || xout == delta)) return fail(TLHIP_EINVAL, "%s: xout must not alias x or delta", who);
+  if (const int rc = check_mx_apart(who, y, {x, delta, norm_w, xout, codes, scales})) return rc;
+  if (xout)
+    if (const int rc = check_mx_apart(who, xout, {norm_w, codes, scales})) return rc;
   const MxRow R{static_cast<const float*>(x), static_cast<const float*>(delta), static_cast<const float*>(norm_w), static_cast<float*>(xout), eps,
                 0, 0, 0};
   const hipError_t e = (gate ? launch_row<kNormed, true> : launch_row<kNormed, false>)(bytes(codes), bytes(scales), N, K, static_cast<float*>(y), R);

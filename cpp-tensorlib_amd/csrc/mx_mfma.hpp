@@ -18,6 +18,8 @@
 // 32 x 448 x 6, which is 0 in f32.
 #pragma once
 
+#include <initializer_list>
+
 #include "gemm_shared.hpp"
 #include "gemv_shared.hpp"
 #include "mx_formats.hpp"
@@ -33,6 +35,13 @@ inline int check_mx_product(const char* who, const void* a, const void* sa, cons
   if (!aligned16(a) || !aligned16(W) || !aligned16(out)) return fail(TLHIP_EINVAL, "%s: elements and result must be 16-byte aligned", who);
   if (M > (1 << 20) || N > (1 << 24) || K > kMxMaxK) return fail(TLHIP_EUNSUPPORTED, "%s: M up to 2^20, N up to 2^24, K up to 65536", who);
   if (M * N > (int64_t)1 << 37) return fail(TLHIP_EUNSUPPORTED, "%s: results of up to 2^37 numbers", who);
+  return TLHIP_OK;
+}
+
+// out: written by some blocks while others read the rest
+inline int check_mx_apart(const char* who, const void* out, std::initializer_list<const void*> operands) {
+  for (const void* p : operands)
+    if (p == out) return fail(TLHIP_EINVAL, "%s: the result must not be written over an operand", who);
   return TLHIP_OK;
 }
 

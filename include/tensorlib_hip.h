@@ -670,7 +670,7 @@ int tlhip_gemm_mxfp4_nt(const void* acodes, const void* ascales, const void* cod
 int tlhip_gemm_mxfp4_nt_parts(const void* acodes, const void* ascales, const void* codes, const void* scales, void* parts,
                               int64_t parts_bytes, int64_t M, int64_t N, int64_t K, int* n_parts);
 /* W = [gate rows | up rows], [2 ff][K]: the gated activation swiglu(A . gate^T, A . up^T) as MXFP8 rows of ff (a multiple of
- * 32), what the down projection reads; the products are never written. */
+ * 32), what the down projection reads. */
 int tlhip_gemm_mxfp4_nt_swiglu(const void* acodes, const void* ascales, const void* codes, const void* scales, void* act_codes,
                                void* act_scales, int64_t M, int64_t ff, int64_t K);
 

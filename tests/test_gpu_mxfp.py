@@ -660,6 +660,31 @@ def test_products_are_deterministic(lib):
         assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
 
 
+def test_results_over_operands_are_refused(lib):
+    """Every product, with its result in the place of each thing it reads (or writes beside it)."""
+    b = lib.empty_bytes(1 << 16)
+    c, n = lib.c, C.c_int(0)
+    p = [b.ptr + 4096 * i for i in range(8)]
+    products = [                                  # call of (operands, result), how many operands
+        (c.tlhip_gemv_mxfp4, lambda o, y: (*o, y, 1, 32), 3),
+        (c.tlhip_gemv_mxfp4_attn, lambda o, y: (o[0], 2, 2, 64, o[1], o[2], y, 1, 128), 3),
+        (c.tlhip_gemv_mxfp4_rmsnorm, lambda o, y: (*o, y, 1, 32, 1e-6), 6),
+        (c.tlhip_gemv_mxfp4_rmsnorm, lambda o, y: (*o[:3], y, *o[3:], 1, 32, 1e-6), 6),              # (the sum's row)
+        (c.tlhip_gemv_mxfp4_rmsnorm_gateup, lambda o, y: (*o, y, 2, 32, 1e-6), 6),
+        (c.tlhip_gemv_mxfp4_rmsnorm_gateup, lambda o, y: (*o[:3], y, *o[3:], 2, 32, 1e-6), 6),
+        (c.tlhip_gemm_mxfp4_nt, lambda o, y: (*o, y, 1, 32, 32), 4),
+        (c.tlhip_gemm_mxfp4_nt_parts, lambda o, y: (*o, y, 4096, 1, 32, 32, C.byref(n)), 4),
+        (c.tlhip_gemm_mxfp4_nt_swiglu, lambda o, y: (*o[:4], y, o[4], 1, 32, 32), 5),
+        (c.tlhip_gemm_mxfp4_nt_swiglu, lambda o, y: (*o, y, 1, 32, 32), 5),
+    ]
+    before = lib.census()
+    for fn, args, operands in products:
+        for i in range(operands):
+            assert fn(*args(p[:operands], p[i])) == -2, (fn.__name__, i)
+            assert lib.last_error().startswith(fn.__name__)
+    assert lib.census() == before
+
+
 def test_refusals(lib):
     b, odd = lib.empty_bytes(1 << 16), C.c_void_p(0)
     p, n = b.ptr, C.c_int(0)
