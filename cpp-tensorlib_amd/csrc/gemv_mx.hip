@@ -743,7 +743,7 @@ extern "C" {
 int tlhip_gemv_mxfp4(const void* a, const void* codes, const void* scales, void* y, int64_t N, int64_t K) {
   TLHIP_REQUIRE_READY();
   const char* who = "tlhip_gemv_mxfp4";
-  if (const int rc = check_mx_product(who, a, scales, codes, scales, y, 1, N, K)) return rc;
+  if (const int rc = check_mx_product(who, a, scales, codes, scales, y, 1, N, K, 4)) return rc;
   if (const int rc = check_mx_apart(who, y, {a, codes, scales})) return rc;
   const MxRow R{static_cast<const float*>(a), nullptr, nullptr, nullptr, 0.f, 0, 0, 0};
   const hipError_t e = launch_row<kFloat, false>(bytes(codes), bytes(scales), N, K, static_cast<float*>(y), R);
@@ -755,7 +755,7 @@ int tlhip_gemv_mxfp4_attn(const void* parts, int64_t n_parts, int64_t heads, int
                           int64_t N, int64_t K) {
   TLHIP_REQUIRE_READY();
   const char* who = "tlhip_gemv_mxfp4_attn";
-  if (const int rc = check_mx_product(who, parts, scales, codes, scales, y, 1, N, K)) return rc;
+  if (const int rc = check_mx_product(who, parts, scales, codes, scales, y, 1, N, K, 4)) return rc;
   if (const int rc = check_attn_merge(parts, n_parts, heads, head_dim, K, who)) return rc;
   if (const int rc = check_mx_apart(who, y, {parts, codes, scales})) return rc;
   const MxRow R{static_cast<const float*>(parts), nullptr, nullptr, nullptr, 0.f, (int)n_parts, (int)heads, (int)head_dim};
@@ -766,7 +766,7 @@ int tlhip_gemv_mxfp4_attn(const void* parts, int64_t n_parts, int64_t heads, int
 
 static int normed(const char* who, const void* x, const void* delta, const void* norm_w, void* xout, const void* codes, const void* scales, void* y,
                   int64_t N, int64_t K, float eps, bool gate) {
-  if (const int rc = check_mx_product(who, x, scales, codes, scales, y, 1, N, K)) return rc;
+  if (const int rc = check_mx_product(who, x, scales, codes, scales, y, 1, N, K, 4)) return rc;
   if (!norm_w) return fail(TLHIP_EINVAL, "%s: null pointer", who);
   if (!aligned16(delta) || !aligned16(norm_w) || !aligned16(xout)) return fail(TLHIP_EINVAL, "%s: delta, norm_w and xout must be 16-byte aligned", who);
   if (xout && (xout == x || xout == delta)) return fail(TLHIP_EINVAL, "%s: xout must not alias x or delta", who);

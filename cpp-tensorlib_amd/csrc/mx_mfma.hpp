@@ -26,13 +26,15 @@
 
 namespace tlhip {
 
-// Arguments of a product, as its entry point `who` checks them. K: what the weight's scales of 16 rows leave room for in LDS.
+// Arguments of a product, as its entry point `who` checks them. K: what the weight's scales of 16 rows leave room for in LDS. align: of
+// the result's address, 4 where it is stored number by number.
 constexpr int64_t kMxMaxK = 65536;
 inline int check_mx_product(const char* who, const void* a, const void* sa, const void* W, const void* sw, const void* out, int64_t M, int64_t N,
-                            int64_t K) {
+                            int64_t K, int align = 16) {
   if (!a || !sa || !W || !sw || !out) return fail(TLHIP_EINVAL, "%s: null pointer", who);
   if (M <= 0 || N <= 0 || !mx_row(K)) return fail(TLHIP_EINVAL, "%s: need M, N > 0, K a positive multiple of 32", who);
-  if (!aligned16(a) || !aligned16(W) || !aligned16(out)) return fail(TLHIP_EINVAL, "%s: elements and result must be 16-byte aligned", who);
+  if (!aligned16(a) || !aligned16(W)) return fail(TLHIP_EINVAL, "%s: elements must be 16-byte aligned", who);
+  if (reinterpret_cast<uintptr_t>(out) % align) return fail(TLHIP_EINVAL, "%s: the result must be %d-byte aligned", who, align);
   if (M > (1 << 20) || N > (1 << 24) || K > kMxMaxK) return fail(TLHIP_EUNSUPPORTED, "%s: M up to 2^20, N up to 2^24, K up to 65536", who);
   if (M * N > (int64_t)1 << 37) return fail(TLHIP_EUNSUPPORTED, "%s: results of up to 2^37 numbers", who);
   return TLHIP_OK;

@@ -637,9 +637,9 @@ int tlhip_latent_attn_run(const void* u, int64_t ldu, const void* q, int64_t ldq
  * scales [rows][K/32] bytes in both. Rows are dense and K is a multiple of 32, so rows of two matrices of the same K can be stacked.
  * Rounding a block: s = floor(log2(largest magnitude)) + 127 - 2 (MXFP4) or - 8 (MXFP8), at least 0; every element is the value
  * over 2^(s - 127), rounded to nearest, ties to even, magnitudes beyond the type's largest becoming that. A block that holds
- * an infinity or a NaN gets the scale 255 and elements 0. What is written must not overlap what is read. Elements must be
- * 16-byte aligned, scales need no alignment. Products take M up to 2^20, N up to 2^24, K up to 65536 and results of up to
- * 2^37 numbers. */
+ * an infinity or a NaN gets the scale 255 and elements 0. What is written must not overlap what is read. Elements, f32 rows and
+ * results must be 16-byte aligned, a decode product's result 4, scales need no alignment. Products take M up to 2^20, N up to
+ * 2^24, K up to 65536 and results of up to 2^37 numbers. */
 /* rows of TLHIP_T_F32, _F16 or _BF16 as a model file holds them -> MXFP4 */
 int tlhip_quantize_mxfp4(const void* src, int src_type, void* codes, void* scales, int64_t rows, int64_t K);
 /* f32 rows -> MXFP8 */

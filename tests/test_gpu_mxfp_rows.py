@@ -1,0 +1,53 @@
+"""Decode products over MXFP4 weights one row after the other: results that lie behind one another at any multiple of four bytes,
+as the logits of several rows of a vocabulary do."""
+import importlib
+
+import numpy as np
+import pytest
+
+import mx_oracle as mx
+from test_gpu_gguf import SMALL, WIDE_HEAD, synth_weights
+from test_gpu_mxfp import activations, product_bound, rng, upload_rows, weight
+from test_gpu_mxfp_model import opened, tokens_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dims,vocab", [(SMALL, 1001), (SMALL, 1002), (WIDE_HEAD, 323)])
+def test_logits_of_several_rows_of_any_vocabulary(tmp_path, dims, vocab):
+    """Rows of logits that no 16 bytes divide: each is what it is when it is asked for alone."""
+    model = importlib.import_module("cpp-tensorlib_amd.model")
+    d = dict(dims, vocab=vocab)
+    path, ids, want = opened(tmp_path, d, synth_weights(d, seed=31)), tokens_of(d, 30, 37), [0, 7, 8, 29]
+    m = model.Model.open(path, max_ctx=d["max_ctx"], mxfp4=True)
+    many = m.feed(ids, want=want)
+    assert many.shape == (4, vocab)
+    for i, t in enumerate(want):
+        m.reset()
+        assert np.array_equal(m.feed(ids, want=[t])[0], many[i])
+    m.close()
+
+
+# a row of the weight in the vector unit, in tiles of 16, in blocks that walk the tiles
+@pytest.mark.parametrize("N,K", [(5, 896), (35, 160), (16640, 2048)])
+@pytest.mark.parametrize("off", [4, 8, 12])
+def test_results_at_any_number(lib, N, K, off):
+    r = rng(41, N, K)
+    x, (wc, wsc) = activations(r, 1, K), weight(r, N, K)
+    bufs, out, dx, nw = upload_rows(lib, wc, wsc, True), lib.empty_bytes(4 * N + 32), lib.to_device(x), lib.to_device(np.ones(K, np.float32))
+    w, x64 = mx.values(wc, wsc, True), x[0].astype(np.float64)
+    big = np.abs(x64).reshape(-1, 32).max(-1).repeat(32)
+    h = x64 / np.sqrt((x64 * x64).mean() + 1e-6)
+    plain = w @ x64, product_bound(x64[None], w, K)[0] + 2.0 ** -38 * (np.abs(w) @ big)
+    normed = w @ h, product_bound(h[None], w, K)[0] + (K / 64 + 20) * 2.0 ** -24 * (np.abs(w) @ np.abs(h))
+    for call, (want, bound) in ((lambda: lib.gemv_mxfp4(dx, *bufs, out, N, K), plain),
+                                (lambda: lib.gemv_mxfp4_rmsnorm(dx, None, nw, None, *bufs, out, N, K, 1e-6), normed)):
+        lib._chk(lib.c.tlhip_fill_u32(out.ptr, 0xa5a5a5a5, N + 8))
+        out.ptr += off
+        call()
+        out.ptr -= off
+        got = out.numpy(np.uint8)
+        assert (got[:off] == 0xa5).all() and (got[off + 4 * N:] == 0xa5).all(), "wrote beside the result"
+        assert (np.abs(got[off:off + 4 * N].copy().view(np.float32) - want) <= bound).all()
+    for b in bufs + (out, dx, nw):
+        b.free()
