@@ -280,9 +280,14 @@ int tlhip_rmsnorm_res_mxfp8(const void* x, const void* parts, int64_t S, const v
     return fail(TLHIP_EUNSUPPORTED, "%s: at most 64 parts, 2^20 rows of 32768", who);
   if (!aligned16(x) || !aligned16(parts) || !aligned16(w) || !aligned16(xout) || !aligned16(codes))
     return fail(TLHIP_EINVAL, "%s: x, parts, w, xout and codes must be 16-byte aligned", who);
-  if (S > 0 && xout == parts) return fail(TLHIP_EINVAL, "%s: xout must not alias the parts", who);
-  if (codes == x || codes == xout || codes == w || codes == scales || (S > 0 && codes == parts) || scales == x || scales == xout)
-    return fail(TLHIP_EINVAL, "%s: codes and scales must not be x, xout, w, the parts or the same", who);
+  // a row's block writes while the blocks of other rows read: xout may be x, of which each block has its own row, and nothing else
+  const void *read[] = {x, w, S > 0 ? parts : nullptr}, *written[] = {xout, codes, scales};
+  for (int i = 0; i < 3; i++) {
+    for (int j = i == 0 ? 1 : 0; j < 3; j++)
+      if (written[i] && written[i] == read[j]) return fail(TLHIP_EINVAL, "%s: what is written must not be what is read, but xout x", who);
+    for (int j = 0; j < i; j++)
+      if (written[i] == written[j]) return fail(TLHIP_EINVAL, "%s: xout, codes and scales must not be the same", who);
+  }
   const int64_t eights = n / 8, V = eights <= 1024 ? 1 : eights <= 2048 ? 2 : 4, threads = ((eights + V - 1) / V + 63) / 64 * 64;
   const auto kernel = V == 1 ? rmsnorm_mxfp8_kernel<1> : V == 2 ? rmsnorm_mxfp8_kernel<2> : rmsnorm_mxfp8_kernel<4>;
   kernel<<<dim3((unsigned)rows), dim3((unsigned)threads), 0, ctx().stream>>>(

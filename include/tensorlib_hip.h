@@ -648,7 +648,7 @@ int tlhip_quantize_mxfp8(const void* x, void* codes, void* scales, int64_t rows,
 int tlhip_dequantize_mxfp4(const void* codes, const void* scales, void* dst, int dst_type, int64_t rows, int64_t K);
 int tlhip_dequantize_mxfp8(const void* codes, const void* scales, void* dst, int dst_type, int64_t rows, int64_t K);
 /* xout = x + (parts[0] + ... + parts[S-1]) in f32, ascending, parts [S][rows][n] (S = 0: none, parts may be NULL);
- * h = xout / sqrt(mean(xout^2) + eps) * w in 64 bits, rounded to f32, then to MXFP8. xout may be NULL, or x; not the parts.
+ * h = xout / sqrt(mean(xout^2) + eps) * w in 64 bits, rounded to f32, then to MXFP8. xout may be NULL, or x.
  * n up to 32768, S up to 64, rows up to 2^20. A row's bytes do not depend on how many rows there are. */
 int tlhip_rmsnorm_res_mxfp8(const void* x, const void* parts, int64_t S, const void* w, void* xout, void* codes, void* scales,
                             int64_t n, float eps, int64_t rows);
