@@ -125,6 +125,18 @@ __device__ __forceinline__ void put_digits(char* lds, int lane, float4 x) {
 }
 
 __host__ __device__ constexpr int rows_sums(int tiles, int waves) { return waves * (tiles * 1024 + 4); }
+// Where the scales of mx_rows_kernel's blocks begin in LDS, 16 bytes of them being put there at a time: behind the sums, or the digits
+__host__ __device__ constexpr int rows_scales(int src, int tiles, int waves) {
+  const int sums = rows_sums(tiles, waves), digits = src == kCodes ? 0 : waves * kUnitLds;
+  return whole_16(sums > digits ? sums : digits);
+}
+constexpr bool rows_scales_whole() {
+  for (int tiles = 1; tiles <= 4; tiles++)
+    for (int waves = 1; waves <= 16; waves++)
+      if (rows_scales(kCodes, tiles, waves) % 16 || rows_scales(kFloat, tiles, waves) % 16) return false;
+  return true;
+}
+static_assert(rows_scales_whole(), "16-byte stores");
 
 // The sums of a feature's twelve digits, which lie in lanes 0 .. 11 of the sixteen that have it: lane i gets feature i of its four
 __device__ __forceinline__ float join_digits(const v4f& c, int r) {
@@ -212,7 +224,7 @@ __global__ __launch_bounds__(SRC == kCodes ? 512 : 1024, 2) void mx_rows_kernel(
   for (int f = 0; f < NF; f++) c[f] = v4f{0.f, 0.f, 0.f, 0.f};
   float ss = 0.f;
   char* const mine = lds + wave * kUnitLds;
-  const uint8_t* const run = reinterpret_cast<const uint8_t*>(lds) + (SRC == kCodes ? rows_sums(NF, waves) : max(rows_sums(NF, waves), waves * kUnitLds));
+  const uint8_t* const run = reinterpret_cast<const uint8_t*>(lds) + rows_scales(SRC, NF, waves);
   const auto multiply = [&](Unit& q, int u) {
     if constexpr (SRC != kCodes) {
       const bool live = 256 * u + 4 * lane < K;
@@ -344,7 +356,7 @@ template <int SRC, int NF, bool GATED>
 static hipError_t launch_rows(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N, int64_t K, int KW,
                               int waves, float* C, uint8_t* codes, uint8_t* scales, const MxRow& R) {
   constexpr int kTile = GATED ? 8 * NF : 16 * NF;
-  const int lds = std::max(SRC == kCodes ? 0 : waves * kUnitLds, rows_sums(NF, waves)) + (GATED ? 2 : 1) * whole_16((int)(waves / KW * kTile * (K / kMxBlock)));
+  const int lds = rows_scales(SRC, NF, waves) + (GATED ? 2 : 1) * whole_16((int)(waves / KW * kTile * (K / kMxBlock)));
   const auto kernel = mx_rows_kernel<SRC, NF, GATED>;
   if (const hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), lds); e != hipSuccess) return e;
   const int64_t per_block = (int64_t)kTile * (waves / KW);
