@@ -189,16 +189,21 @@ __global__ __launch_bounds__(64 * WF * WT, WPE) void mx_tile_kernel(const uint8_
   }
 }
 
+// Blocks of a launch, each 256 threads, which a grid's x counts in 32 bits. Results of up to 2^37 numbers are at most 2^23 tiles of the
+// largest kind, half as many features with the gate, and those that the ends of its rows and columns add.
+constexpr int64_t kMostTiles = ((int64_t)1 << 24) - 1;
+
 template <int WF, int WT, int NF, int NT, int WPE, bool GATED>
 static hipError_t launch_tiles(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N, int64_t K, int parts,
                                int64_t apart, float* C, uint8_t* codes, uint8_t* scales) {
   constexpr int TF = 16 * NF * WF / (GATED ? 2 : 1), TT = 16 * NT * WT;
   constexpr int lds = 2 * (16 * NF * WF * 68 + TT * 132);
   static_assert(lds <= 160 * 1024, "LDS");
+  static_assert(64 * WF * WT == 256, "what kMostTiles counts");
   MxTiles P;
   P.tokens = (int)((M + TT - 1) / TT);
   const int64_t count = (N + TF - 1) / TF * P.tokens;
-  if (count > (1 << 24) / (WF * WT)) return hipErrorInvalidValue;   // (a grid's x counts threads in 32 bits)
+  if (count > kMostTiles) return hipErrorInvalidValue;
   P.count = (int)count;
   const int all = (int)((K + 127) / 128);
   P.steps = (all + parts - 1) / parts;
@@ -231,6 +236,7 @@ static MxPlan plan_tiles(int64_t M, int64_t N, int64_t K, int64_t max_parts, boo
   for (int v = 0; v < kVariants; v++) {
     const int64_t features = kVariant[v].features / (gated ? 2 : 1);
     const int64_t tiles = (N + features - 1) / features * ((M + kVariant[v].tokens - 1) / kVariant[v].tokens);
+    if (tiles > kMostTiles) continue;
     for (const int64_t S : {1, 2, 3, 4, 6, 8, 12, 16}) {
       if (S > 1 && (S > max_parts || steps / S < 2)) break;
       const int64_t each = (steps + S - 1) / S, parts = (steps + each - 1) / each;

@@ -1,5 +1,5 @@
-"""Decode products over MXFP4 weights one row after the other: results that lie behind one another at any multiple of four bytes,
-as the logits of several rows of a vocabulary do."""
+"""Products over MXFP4 weights whose results lie where, or are as large as, no ordinary ones: rows of logits behind one another at any
+multiple of four bytes, results of more than 2^36 numbers."""
 import importlib
 
 import numpy as np
@@ -7,7 +7,7 @@ import pytest
 
 import mx_oracle as mx
 from test_gpu_gguf import SMALL, WIDE_HEAD, synth_weights
-from test_gpu_mxfp import activations, product_bound, rng, upload_rows, weight
+from test_gpu_mxfp import activations, check_gated, product_bound, rng, rows8, upload_rows, weight
 from test_gpu_mxfp_model import opened, tokens_of
 
 pytestmark = pytest.mark.gpu
@@ -50,4 +50,29 @@ def test_results_at_any_number(lib, N, K, off):
         assert (got[:off] == 0xa5).all() and (got[off + 4 * N:] == 0xa5).all(), "wrote beside the result"
         assert (np.abs(got[off:off + 4 * N].copy().view(np.float32) - want) <= bound).all()
     for b in bufs + (out, dx, nw):
+        b.free()
+
+
+def test_gated_result_of_more_than_2_to_the_36_numbers(lib):
+    """64 GB of elements, in more than 2^22 tiles; rows from all over it, the first and the last, against 64 bits."""
+    r, M, ff, K = rng(43), 1 << 20, 65568, 32
+    (ac, asc), (wc, wsc) = rows8(r, M, K), weight(r, 2 * ff, K)
+    wsc = (wsc + 3).astype(np.uint8)
+    bufs = upload_rows(lib, ac, asc) + upload_rows(lib, wc, wsc, True)
+    codes, scales = lib.empty_bytes(M * ff + 256), lib.empty_bytes(M * ff // 32 + 256)
+    for b, n in ((codes, M * ff), (scales, M * ff // 32)):
+        lib._chk(lib.c.tlhip_fill_u32(b.ptr + n, 0xa5a5a5a5, 64))
+    lib.gemm_mxfp4_nt_swiglu(*bufs, codes, scales, M, ff, K)
+
+    def read(ptr, n):
+        out = np.empty(n, np.uint8)
+        lib._chk(lib.c.tlhip_memcpy_d2h(out.ctypes.data, ptr, n))
+        return out
+
+    rows = np.unique(np.concatenate([[0, 1, 127, 128, M // 2 - 1, M // 2, M - 129, M - 128, M - 2, M - 1], r.integers(0, M, 8)]))
+    got_c = np.stack([read(codes.ptr + int(m) * ff, ff) for m in rows])
+    got_s = np.stack([read(scales.ptr + int(m) * (ff // 32), ff // 32) for m in rows])
+    check_gated(got_c, got_s, mx.values(ac[rows], asc[rows], False), mx.values(wc, wsc, True), K)
+    assert (read(codes.ptr + M * ff, 256) == 0xa5).all() and (read(scales.ptr + M * ff // 32, 256) == 0xa5).all(), "wrote behind the result"
+    for b in bufs + (codes, scales):
         b.free()
