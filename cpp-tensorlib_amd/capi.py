@@ -171,6 +171,8 @@ SIGNATURES = {
     "tlhip_tune_attn_prefill": (cint, [cint]),
     "tlhip_tune_gemm_planes": (cint, [cint]),
     "tlhip_plan_gemm_bf16": (cint, [i64, i64, i64, cint, cint, C.POINTER(cint)]),
+    "tlhip_plan_gemv_mxfp4": (cint, [i64, i64, cint, cint, C.POINTER(cint)]),
+    "tlhip_plan_gemm_mxfp4": (cint, [i64, i64, i64, cint, cint, C.POINTER(cint)]),
     "tlhip_plan_gemm_f16w": (cint, [i64, i64, i64, cint, cint, P]),
     "tlhip_tune_reset": (cint, []),
     "tlhip_bench_copy": (cint, [P, P, sz, cint]),
@@ -758,6 +760,18 @@ class TlHip:
         v = (i64 * 8)()
         self._chk(self.c.tlhip_plan_gemm_f16w(M, N, K, int(gated), parts, v))
         return [tuple(v[4 * i:4 * i + 4]) for i in range(2) if v[4 * i] > 0]
+
+    def plan_gemv_mxfp4(self, N, K, producer=0, gated=False):
+        """(0: vector unit, 1: blocks that walk tiles, 2: a block for each set; rows of a wavefront; wavefronts a row, a block; units of 256 k)"""
+        v = (cint * 5)()
+        self._chk(self.c.tlhip_plan_gemv_mxfp4(N, K, producer, int(gated), v))
+        return tuple(v)
+
+    def plan_gemm_mxfp4(self, M, N, K, gated=False, parts=0):
+        """(blocks of 16 rows?, features and rows of a block or tile, K parts, the gate by a launch of its own?)"""
+        v = (cint * 5)()
+        self._chk(self.c.tlhip_plan_gemm_mxfp4(M, N, K, int(gated), parts, v))
+        return tuple(v)
 
     def tune_reset(self):
         self._chk(self.c.tlhip_tune_reset())

@@ -249,6 +249,32 @@ static MxPlan plan_tiles(int64_t M, int64_t N, int64_t K, int64_t max_parts, boo
   return best;
 }
 
+// A product without the gate: rows of 16 a block, or tiles
+struct MxProduct { bool rows; MxPlan tiles; };
+static MxProduct plan_product(int64_t M, int64_t N, int64_t K, int64_t max_parts, bool own_sum) {
+  const MxPlan tiles = plan_tiles(M, N, K, max_parts, false, own_sum);
+  return MxProduct{mx_few_rows_us(M, N, K) < tiles.us, tiles};
+}
+
+// A gated product. apart: the products, then a launch that gates them; of few tiles over a long K, gate and up products in parts
+// that it adds up (us so, and in one launch, each with the result read back, 2 to 3 of them: 282 x 32 x 11552
+// 12.5, 55.9; 310 x 832 x 8128 26.5, 49.9). Of few rows the products are then those of 16 rows
+// a block, or of tiles in parts, as their estimates say; up to 16 rows the one launch has blocks of 32 gate and 32 up rows (12 x 32 x 10368
+// 11.5, 16.3; 7 x 1792 x 5440 9.1, 11.7; 16 x 512 x 1536 7.7, 8.1; 1024 7.6, 7.9; 16 x 6144 x 3584, where those fill the CUs, 14.0, 11.3).
+// room: for the products.
+struct MxGated { bool apart, rows; MxPlan tiles; };
+static MxGated plan_gated(int64_t M, int64_t ff, int64_t K, bool room) {
+  const bool few = M <= kMxFewRows, fits = few && mx_few_rows_fit(ff, K, true);
+  const MxPlan one = plan_tiles(M, ff, K, 1, true, false);
+  MxPlan two = plan_tiles(M, 2 * ff, K, 16, false, false);
+  const double rows_us = mx_few_rows_us(M, 2 * ff, K), whole = 4.0 * (double)M * (double)ff * 4.0 / 5.4e6;    // (of one part, written and read)
+  if (two.parts == 1) two.us += whole;
+  const bool rows = rows_us + whole < two.us;
+  if (rows) two = MxPlan{0, 1, rows_us + whole};
+  const bool apart = few ? !fits || (K >= 1536 && ff / kMxBlock <= cu_count() / 2) : two.us + 2.2 < one.us;
+  return apart && room ? MxGated{true, rows, two} : MxGated{false, fits, one};
+}
+
 static hipError_t launch_plan(const MxPlan& P, const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N,
                               int64_t K, int64_t apart, float* C, uint8_t* codes, uint8_t* scales) {
   if (codes) {
@@ -318,13 +344,13 @@ int tlhip_gemm_mxfp4_nt_parts(const void* acodes, const void* ascales, const voi
   if (!n_parts) return fail(TLHIP_EINVAL, "%s: null pointer", who);
   if (parts_bytes < M * N * 4) return fail(TLHIP_EINVAL, "%s: the parts need M * N * 4 bytes at least", who);
   hipError_t e;
-  const MxPlan P = plan_tiles(M, N, K, parts_bytes / (M * N * 4), false, false);
-  if (mx_few_rows_us(M, N, K) < P.us) {
+  const MxProduct P = plan_product(M, N, K, parts_bytes / (M * N * 4), false);
+  if (P.rows) {
     *n_parts = 1;
     e = launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, static_cast<float*>(parts), nullptr, nullptr);
   } else {
-    *n_parts = P.parts;
-    e = launch_plan(P, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, M * N, static_cast<float*>(parts), nullptr, nullptr);
+    *n_parts = P.tiles.parts;
+    e = launch_plan(P.tiles, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, M * N, static_cast<float*>(parts), nullptr, nullptr);
   }
   if (e != hipSuccess) return hip_fail(e, who);
   TLHIP_CHECK_LAUNCH(TLHIP_C_GEMM_MXFP4);
@@ -337,8 +363,9 @@ int tlhip_gemm_mxfp4_nt(const void* acodes, const void* ascales, const void* cod
   if (const int rc = check_mx_product(who, acodes, ascales, codes, scales, C, M, N, K)) return rc;
   if (const int rc = check_mx_apart(who, C, {acodes, ascales, codes, scales})) return rc;
   hipError_t e;
-  MxPlan P = plan_tiles(M, N, K, 16, false, true);
-  if (mx_few_rows_us(M, N, K) < P.us) {
+  const MxProduct product = plan_product(M, N, K, 16, true);
+  MxPlan P = product.tiles;
+  if (product.rows) {
     e = launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, N, K, static_cast<float*>(C), nullptr, nullptr);
   } else {
     const int64_t apart = (M * N + 3) & ~(int64_t)3;
@@ -369,34 +396,37 @@ int tlhip_gemm_mxfp4_nt_swiglu(const void* acodes, const void* ascales, const vo
   if (const int rc = check_mx_apart(who, act_codes, {acodes, ascales, codes, scales, act_scales})) return rc;
   if (const int rc = check_mx_apart(who, act_scales, {acodes, ascales, codes, scales})) return rc;
   uint8_t *qc = static_cast<uint8_t*>(act_codes), *qs = static_cast<uint8_t*>(act_scales);
-  // Few tiles over a long K: gate and up products in parts, and a launch that adds them up and gates (us so, and in one launch, each with the
-  // result read back, 2 to 3 of them: 282 x 32 x 11552
-  // 12.5, 55.9; 310 x 832 x 8128 26.5, 49.9). Of few rows the products are then those of 16 rows
-  // a block, or of tiles in parts, as their estimates say; up to 16 rows the one launch has blocks of 32 gate and 32 up rows (12 x 32 x 10368
-  // 11.5, 16.3; 7 x 1792 x 5440 9.1, 11.7; 16 x 512 x 1536 7.7, 8.1; 1024 7.6, 7.9; 16 x 6144 x 3584, where those fill the CUs, 14.0, 11.3).
-  const bool few = M <= kMxFewRows;
-  const MxPlan one = plan_tiles(M, ff, K, 1, true, false);
-  MxPlan two = plan_tiles(M, 2 * ff, K, 16, false, false);
-  const double rows_us = mx_few_rows_us(M, 2 * ff, K), whole = 4.0 * (double)M * (double)ff * 4.0 / 5.4e6;    // (of one part, written and read)
-  if (two.parts == 1) two.us += whole;
-  const bool rows = rows_us + whole < two.us;
-  if (rows) two = MxPlan{0, 1, rows_us + whole};
-  const bool apart = few ? !mx_few_rows_fit(ff, K, true) || (K >= 1536 && ff / kMxBlock <= cu_count() / 2) : two.us + 2.2 < one.us;
-  float* const parts = apart ? static_cast<float*>(scratch((size_t)two.parts * M * 2 * ff * 4)) : nullptr;    // (a recording may not grow it)
+  MxGated P = plan_gated(M, ff, K, true);
+  float* const parts = P.apart ? static_cast<float*>(scratch((size_t)P.tiles.parts * M * 2 * ff * 4)) : nullptr;
+  if (P.apart && !parts) P = plan_gated(M, ff, K, false);       // (a recording may not grow it)
   hipError_t e;
-  if (parts) {
-    e = rows ? launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, 2 * ff, K, parts, nullptr, nullptr)
-             : launch_plan(two, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, 2 * ff, K, M * 2 * ff, parts, nullptr, nullptr);
+  if (P.apart) {
+    e = P.rows ? launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, 2 * ff, K, parts, nullptr, nullptr)
+               : launch_plan(P.tiles, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, 2 * ff, K, M * 2 * ff, parts, nullptr, nullptr);
     if (e == hipSuccess)
       mx_gate_sum_kernel<<<dim3((unsigned)((M * (ff / 4) + 255) / 256)), dim3(256), 0, ctx().stream>>>(reinterpret_cast<const float4*>(parts), qc, qs, M,
-                                                                                                       (int)(ff / 4), two.parts);
-  } else if (few && mx_few_rows_fit(ff, K, true)) {
+                                                                                                       (int)(ff / 4), P.tiles.parts);
+  } else if (P.rows) {
     e = launch_mx_few_rows(bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, ff, K, nullptr, qc, qs);
   } else {
-    e = launch_plan(one, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, ff, K, 0, nullptr, qc, qs);
+    e = launch_plan(P.tiles, bytes(acodes), bytes(ascales), bytes(codes), bytes(scales), M, ff, K, 0, nullptr, qc, qs);
   }
   if (e != hipSuccess) return hip_fail(e, who);
   TLHIP_CHECK_LAUNCH(TLHIP_C_GEMM_MXFP4);
+}
+
+int tlhip_plan_gemm_mxfp4(int64_t M, int64_t N, int64_t K, int gated, int parts, int plan[5]) {
+  const char* who = "tlhip_plan_gemm_mxfp4";
+  if (!plan || M <= 0 || N <= 0 || !mx_row(K) || parts < 0 || (gated && (parts || !mx_row(N)))) return fail(TLHIP_EINVAL, "%s: bad arguments", who);
+  if (M > (1 << 20) || N > (1 << 24) || K > kMxMaxK || M * N > (int64_t)1 << 37) return fail(TLHIP_EUNSUPPORTED, "%s: dimension too large", who);
+  const MxGated g = gated ? plan_gated(M, N, K, true) : MxGated{};
+  const MxProduct p = gated ? MxProduct{g.rows, g.tiles} : plan_product(M, N, K, parts ? parts : 16, parts == 0);
+  plan[0] = p.rows;
+  plan[1] = !p.rows ? kVariant[p.tiles.variant].features : gated && !g.apart ? 64 : 16 * mx_few_rows_tiles(M, gated ? 2 * N : N, K);
+  plan[2] = p.rows ? 16 : kVariant[p.tiles.variant].tokens;
+  plan[3] = p.rows ? 1 : p.tiles.parts;
+  plan[4] = g.apart;
+  return TLHIP_OK;
 }
 
 }  // extern "C"

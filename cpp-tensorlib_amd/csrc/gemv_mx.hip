@@ -698,27 +698,44 @@ static hipError_t launch_row_small(const uint8_t* W, const uint8_t* sw, int64_t 
 //     than CUs, which hold one of sixteen (16384 x 8192 17.2, 19.5; 28672 x 8192 normed 30.4, 38.5; 32768 x 5120 gated 21.5, 30.1);
 //   32 rows a block where there are more tiles of 16 than CUs (4608 x 3584 5.1, 16: 5.9; gated 6.6, 8.8; 3584 x 18944 12.9, 16: 9.8), and while
 //     the scales of their rows leave room in LDS.
-template <int SRC, bool GATED>
-static hipError_t launch_row(const uint8_t* W, const uint8_t* sw, int64_t N, int64_t K, float* y, const MxRow& R) {
+enum { kRowVector = 0, kRowWalk = 1, kRowTiles = 2 };
+struct RowPlan {
+  int form;                  // mx_row_small_kernel, mx_row_tiles_kernel, mx_rows_kernel
+  int rows;                  // of the weight, that a wavefront has at a time
+  int KW, waves;             // wavefronts that share a row, of a block
+  int units;                 // kRowWalk: of 256 k, that a wavefront has
+};
+static RowPlan plan_row(int64_t N, int64_t K, int src, bool gated) {
   const int64_t nb = K / kMxBlock, units = (nb + 7) / 8, cus = cu_count();
   const int KW = units <= 1 ? 1 : units <= 2 ? 2 : units <= 4 ? 4 : 8;
-  const int64_t rows = (GATED ? 8 : 16) * (8 / KW);          // of a tile, gate rows if gated
-  const int64_t all = GATED ? 2 * N : N;                     // rows of the weight
-  if constexpr (SRC == kFloat) {
-    if ((all * K <= (int64_t)20 << 20 || all <= 4 * cus) && K >= 512 && (K >= 896 || all <= 64 * cus))
-      return launch_row_small<SRC, 4, false>(W, sw, N, K, (int)std::min<int64_t>(16, (K + 1023) / 1024), 1, y, R);
+  const int64_t rows = (gated ? 8 : 16) * (8 / KW);          // of a tile, gate rows if gated
+  const int64_t all = gated ? 2 * N : N;                     // rows of the weight
+  const int kw = (int)std::min<int64_t>(16, (K + 1023) / 1024);
+  if (src == kFloat) {
+    if ((all * K <= (int64_t)20 << 20 || all <= 4 * cus) && K >= 512 && (K >= 896 || all <= 64 * cus)) return RowPlan{kRowVector, 4, kw, kw, 0};
   } else {
-    if ((all * K <= (int64_t)9 << 20 || all <= 4 * cus) && K >= 512 && K <= 32768) {
-      const int kw = (int)std::min<int64_t>(16, (K + 1023) / 1024), fw = kw <= 8 ? 2 : 1;
-      return (all <= 2 * fw * cus ? launch_row_small<SRC, 2, GATED> : launch_row_small<SRC, 4, GATED>)(W, sw, N, K, kw, fw, y, R);
-    }
+    const int sets = kw <= 8 ? 2 : 1;
+    if ((all * K <= (int64_t)9 << 20 || all <= 4 * cus) && K >= 512 && K <= 32768)
+      return RowPlan{kRowVector, all <= 2 * sets * cus ? 2 : 4, kw, kw * sets, 0};
+  }
+  if (src != kMerged && units <= 16 && N % 16 == 0 && N > (units > 12 ? 2 : 4) * cus * rows && rows * nb % 16 == 0)
+    return RowPlan{kRowWalk, 16, KW, 8, units <= KW ? 1 : 2};
+  const bool two = all > 16 * cus && nb <= 1024;
+  const int waves = units <= 12 || all > (two ? 32 : 16) * cus ? 8 : 16;
+  return RowPlan{kRowTiles, two ? 32 : 16, units <= 8 ? KW : waves, waves, 0};
+}
+
+template <int SRC, bool GATED>
+static hipError_t launch_row(const uint8_t* W, const uint8_t* sw, int64_t N, int64_t K, float* y, const MxRow& R) {
+  const RowPlan P = plan_row(N, K, SRC, GATED);
+  if (P.form == kRowVector) {
+    if constexpr (SRC == kFloat) return launch_row_small<SRC, 4, false>(W, sw, N, K, P.KW, P.waves / P.KW, y, R);
+    else return (P.rows == 2 ? launch_row_small<SRC, 2, GATED> : launch_row_small<SRC, 4, GATED>)(W, sw, N, K, P.KW, P.waves / P.KW, y, R);
   }
   if constexpr (SRC != kMerged)
-    if (units <= 16 && N % 16 == 0 && N > (units > 12 ? 2 : 4) * cus * rows && rows * nb % 16 == 0)
-      return (units <= KW ? launch_row_tiles<SRC, 1, GATED, 1> : launch_row_tiles<SRC, 1, GATED, 2>)(W, sw, N, K, KW, 2, y, R);
-  const bool two = all > 16 * cus && nb <= 1024;
-  const int waves = units <= 12 || all > (two ? 32 : 16) * cus ? 8 : 16, kw = units <= 8 ? KW : waves;
-  return (two ? launch_rows<SRC, 2, GATED> : launch_rows<SRC, 1, GATED>)(nullptr, nullptr, W, sw, 1, N, K, kw, waves, y, nullptr, nullptr, R);
+    if (P.form == kRowWalk)
+      return (P.units == 1 ? launch_row_tiles<SRC, 1, GATED, 1> : launch_row_tiles<SRC, 1, GATED, 2>)(W, sw, N, K, P.KW, 2, y, R);
+  return (P.rows == 32 ? launch_rows<SRC, 2, GATED> : launch_rows<SRC, 1, GATED>)(nullptr, nullptr, W, sw, 1, N, K, P.KW, P.waves, y, nullptr, nullptr, R);
 }
 
 bool mx_few_rows_fit(int64_t N, int64_t K, bool gated) {
@@ -726,12 +743,12 @@ bool mx_few_rows_fit(int64_t N, int64_t K, bool gated) {
   return !gated || 64 * (K / kMxBlock) <= 120 * 1024;
 }
 // 16 rows of the weight a block, 32 where there would be more blocks than CUs (77 x 896 x 4864 7.4 us, with 16 8.9)
-static int rows_tiles(int64_t M, int64_t N, int64_t K) { return (N + 15) / 16 * ((M + 15) / 16) > cu_count() && K <= 32768 ? 2 : 1; }
+int mx_few_rows_tiles(int64_t M, int64_t N, int64_t K) { return (N + 15) / 16 * ((M + 15) / 16) > cu_count() && K <= 32768 ? 2 : 1; }
 // Up to a block on each CU it takes 2.9 us and 27 ns for each KB that a block reads, of both operands; up to two blocks twice that, beyond which
 // tiles that share what they read are ahead (measured 17 to 256 rows by 896 x 896 to 4608 x 3584: 48 x 896 x 4864 5.6, estimated 6.0, in
 // tiles 6.9; 112 x 1152 x 896 3.7, 3.9, 5.3; 48 x 3584 x 3584 9.7, 9.1, 9.1).
 double mx_few_rows_us(int64_t M, int64_t N, int64_t K) {
-  const int64_t nf = rows_tiles(M, N, K), blocks = (N + 16 * nf - 1) / (16 * nf) * ((M + 15) / 16), cus = cu_count();
+  const int64_t nf = mx_few_rows_tiles(M, N, K), blocks = (N + 16 * nf - 1) / (16 * nf) * ((M + 15) / 16), cus = cu_count();
   if (blocks > 2 * cus) return M <= kMxFewRows ? 0 : 1e30;
   return 2.9 + (double)((blocks + cus - 1) / cus) * (double)(nf * K * 17 / 2 + std::min<int64_t>(M, 16) * K) / 1024 * 0.027;
 }
@@ -740,7 +757,7 @@ hipError_t launch_mx_few_rows(const uint8_t* A, const uint8_t* sa, const uint8_t
   const int64_t units = (K + 255) / 256;
   const int KW = units <= 1 ? 1 : units <= 2 ? 2 : units <= 4 ? 4 : 8;
   if (codes) return launch_rows<kCodes, 4, true>(A, sa, W, sw, M, N, K, KW, KW, C, codes, scales, MxRow{});
-  return (rows_tiles(M, N, K) == 2 ? launch_rows<kCodes, 2, false> : launch_rows<kCodes, 1, false>)(A, sa, W, sw, M, N, K, KW, KW, C, nullptr, nullptr,
+  return (mx_few_rows_tiles(M, N, K) == 2 ? launch_rows<kCodes, 2, false> : launch_rows<kCodes, 1, false>)(A, sa, W, sw, M, N, K, KW, KW, C, nullptr, nullptr,
                                                                                                   MxRow{});
 }
 
@@ -804,6 +821,19 @@ int tlhip_gemv_mxfp4_rmsnorm_gateup(const void* x, const void* delta, const void
   const char* who = "tlhip_gemv_mxfp4_rmsnorm_gateup";
   if (N2 % 2) return fail(TLHIP_EINVAL, "%s: need as many gate rows as up rows", who);
   return normed(who, x, delta, norm_w, xout, codes, scales, act, N2 / 2, K, eps, true);
+}
+
+int tlhip_plan_gemv_mxfp4(int64_t N, int64_t K, int producer, int gated, int plan[5]) {
+  const char* who = "tlhip_plan_gemv_mxfp4";
+  if (!plan || N <= 0 || !mx_row(K) || producer < 0 || producer > 2 || (gated && producer != 1)) return fail(TLHIP_EINVAL, "%s: bad arguments", who);
+  if (N > (1 << 24) || K > kMxMaxK) return fail(TLHIP_EUNSUPPORTED, "%s: dimension too large", who);
+  const RowPlan P = plan_row(N, K, producer == 0 ? kFloat : producer == 1 ? kNormed : kMerged, gated != 0);
+  plan[0] = P.form;
+  plan[1] = P.rows;
+  plan[2] = P.KW;
+  plan[3] = P.waves;
+  plan[4] = P.units;
+  return TLHIP_OK;
 }
 
 }  // extern "C"

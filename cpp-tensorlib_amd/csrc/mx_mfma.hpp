@@ -57,6 +57,7 @@ inline hipError_t allow_lds(const void* kernel, int lds) {
 constexpr int kMxFewRows = 16;
 double mx_few_rows_us(int64_t M, int64_t N, int64_t K);
 bool mx_few_rows_fit(int64_t N, int64_t K, bool gated);
+int mx_few_rows_tiles(int64_t M, int64_t N, int64_t K);      // of 16 features, that a block has
 hipError_t launch_mx_few_rows(const uint8_t* A, const uint8_t* sa, const uint8_t* W, const uint8_t* sw, int64_t M, int64_t N, int64_t K, float* C,
                               uint8_t* codes, uint8_t* scales);
 

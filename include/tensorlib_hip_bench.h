@@ -69,8 +69,17 @@ int tlhip_plan_gemm_f16w(int64_t M, int64_t N, int64_t K, int gated, int parts, 
 /* Which kernel forms a bf16 product (tlhip_gemm_bf16_nt, or gated its _swiglu form with N features; parts > 0: the _parts form with
  * room for so many), its result 16-byte aligned, and how: plan[0] 1 = the kernel of few rows (plan[1], [2]: its row and column tiles
  * of 16 to a block), 0 = tiles of 64 or 128 rows; [3] K splits; [4] the longest chain of 32-k steps that one accumulator sums. On the
- * host alone, as above. Both refuse sizes that the products refuse. */
+ * host alone, as above. These refuse sizes that the products refuse. */
 int tlhip_plan_gemm_bf16(int64_t M, int64_t N, int64_t K, int gated, int parts, int plan[5]);
+/* Which kernel forms a decode product over an MXFP4 weight (producer 0: tlhip_gemv_mxfp4, 1: _rmsnorm, or gated _rmsnorm_gateup with N
+ * gate rows, 2: _attn), and how: plan[0] 0 = the vector unit, 1 = blocks that walk tiles of 16 rows, 2 = a block for each set of tiles;
+ * [1] rows of the weight that a wavefront has at a time; [2] wavefronts that share a row; [3] of a block; [4] with 1: units of 256 k that a
+ * wavefront has, else 0. On the host alone, as above. */
+int tlhip_plan_gemv_mxfp4(int64_t N, int64_t K, int producer, int gated, int plan[5]);
+/* The same of products of MXFP8 rows (tlhip_gemm_mxfp4_nt, or gated its _swiglu form with N features; parts > 0: the _parts form with
+ * room for so many): plan[0] 1 = blocks of 16 rows, 0 = tiles; [1], [2] features (of the weight's rows) and rows of a block or tile; [3]
+ * parts that K is split into; [4] gated: 1 = by a launch of its own behind the products. */
+int tlhip_plan_gemm_mxfp4(int64_t M, int64_t N, int64_t K, int gated, int parts, int plan[5]);
 /* Every override back to the built-in choice (tlhip_tune_gemv_cols included). */
 int tlhip_tune_reset(void);
 
