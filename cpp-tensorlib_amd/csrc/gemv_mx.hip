@@ -16,7 +16,8 @@ namespace tlhip {
 // as e4m3, that many times 2^-9, so a digit is its own code; with the number's sign it is one element of a row of the second operand,
 // digit p in row p under the scale 16^p. The row's twelve sums, which no product's last bit is missing from, are added up at the end. A
 // number keeps all of its 24 bits down to 2^-24 of its block's largest, below that an absolute error of 2^-48 of it. Numbers
-// below 2^-81 are cut at 2^-128; a block with an infinity or a NaN is NaN. Dequantised in the vector unit (1.5 instructions for each
+// below 2^-81 are cut at 2^-128; a block with an infinity or a NaN is NaN. The sums are of y / 256, so that the largest fit: each of the 192 +
+// K / 128 roundings of each of the twelve is 2^-150 at least, 2^-142 of y. Dequantised in the vector unit (1.5 instructions for each
 // weight, the conversion of e2m1 alone nearly three times an FMA) the same product was bound by it.
 //
 // The scales of a block's rows are one run of bytes: copied into LDS whole (a byte loaded by each lane was a request for 16 lines: 70 us

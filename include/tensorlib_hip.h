@@ -653,7 +653,8 @@ int tlhip_dequantize_mxfp8(const void* codes, const void* scales, void* dst, int
 int tlhip_rmsnorm_res_mxfp8(const void* x, const void* parts, int64_t S, const void* w, void* xout, void* codes, void* scales,
                             int64_t n, float eps, int64_t rows);
 /* y[n] = sum_k a[k] W[n][k], a f32, W MXFP4 [N][K], f32 sums: the decode product. A number of a keeps its 24 bits down to 2^-24 of the
- * largest of its block of 32, below that an absolute error of 2^-48 of that (and of 2^-128); an infinity or a NaN in a makes every y NaN. */
+ * largest of its block of 32, below that an absolute error of 2^-48 of that (and of 2^-128); an infinity or a NaN in a makes every y NaN. Sums
+ * are kept over 256: y is off by up to 12 (192 + K / 128) 2^-142 (2^-128 at most) besides, where it is next to the smallest numbers. */
 int tlhip_gemv_mxfp4(const void* a, const void* codes, const void* scales, void* y, int64_t N, int64_t K);
 /* The same with the producers of tlhip_gemv_q4_attn, tlhip_gemv_q4_rmsnorm and tlhip_gemv_q4_rmsnorm_gateup, whose arguments these
  * have. */

@@ -234,10 +234,11 @@ HARD = [(70, 288), (4128, 480), (1671, 12576), (34320, 544), (16432, 1280), (878
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("N,K", HARD)
-@pytest.mark.parametrize("kind", ["spread", "largest", "top", "smallest", "bottom", "one outlier", "blocks apart"])
+@pytest.mark.parametrize("kind", ["spread", "largest", "top", "smallest", "bottom", "results at the bottom", "one outlier", "blocks apart"])
 def test_token_product_of_hard_rows(lib, N, K, kind):
     """f32 sums of the row's numbers as they are: magnitudes all over a block, or over the row's blocks, at both ends of f32, and one
-    that dwarfs its neighbours under weights of zero."""
+    that dwarfs its neighbours under weights of zero. Twelve digits' sums of y / 256 have 192 + K / 128 roundings each, of 2^-150 where
+    they are subnormal."""
     r = rng(106, N, K)
     x, (wc, wsc) = r.standard_normal((1, K)).astype(np.float32), weight(r, min(N, PERIOD), K)
     if kind == "spread":
@@ -255,6 +256,9 @@ def test_token_product_of_hard_rows(lib, N, K, kind):
     elif kind == "bottom":                                 # (largest numbers of 2^-78 to 2^-148)
         x = (x / np.abs(x).max() * 2.0 ** -r.integers(78, 149, K // 32).astype(np.float64).repeat(32)).astype(np.float32)
         wsc = (wsc + 60).astype(np.uint8)
+    elif kind == "results at the bottom":                  # (some of them subnormal)
+        x *= np.float32(2.0 ** -66)
+        wsc = (wsc - 66).astype(np.uint8)
     elif kind == "one outlier":
         x[0, 5::32] = 2.0 ** 20
         wc[:, 5::32] &= 8
@@ -265,7 +269,7 @@ def test_token_product_of_hard_rows(lib, N, K, kind):
     bufs, dx, out = upload_rows(lib, wc[at], wsc[at], True), lib.to_device(x), guarded(lib, 4 * N)
     lib.gemv_mxfp4(dx, *bufs, out, N, K)
     big = np.abs(x64).reshape(-1, 32).max(-1).repeat(32)
-    bound = product_bound(x64[None], w, K)[0] + np.abs(w) @ np.maximum(2.0 ** -48 * big, 2.0 ** -128)
+    bound = product_bound(x64[None], w, K)[0] + np.abs(w) @ np.maximum(2.0 ** -48 * big, 2.0 ** -128) + 12 * (192 + K / 128) * 2.0 ** -142
     assert (np.abs(taken(out, 4 * N, np.float32, (N,)) - spread(w @ x64, N)) <= spread(bound, N)).all()
     for b in bufs + (dx, out):
         b.free()

@@ -1,5 +1,5 @@
 """Products over MXFP4 weights whose results lie where, or are as large as, no ordinary ones: rows of logits behind one another at any
-multiple of four bytes, results of more than 2^36 numbers."""
+multiple of four bytes, results of more than 2^36 numbers, weights of more than one launch of the rounding."""
 import importlib
 
 import numpy as np
@@ -75,4 +75,36 @@ def test_gated_result_of_more_than_2_to_the_36_numbers(lib):
     check_gated(got_c, got_s, mx.values(ac[rows], asc[rows], False), mx.values(wc, wsc, True), K)
     assert (read(codes.ptr + M * ff, 256) == 0xa5).all() and (read(scales.ptr + M * ff // 32, 256) == 0xa5).all(), "wrote behind the result"
     for b in bufs + (codes, scales):
+        b.free()
+
+
+def test_rounding_of_more_than_one_launch(lib):
+    """More than 2^34 numbers, 2^31 lanes of eight, which a grid counts: ones, but random rows at the first launch's end and at the last."""
+    r, K = rng(47), 65536
+    rows = (1 << 18) + 40
+    src, codes, scales = lib.empty_bytes(rows * K * 2), lib.empty_bytes(rows * K // 2), lib.empty_bytes(rows * K // 32)
+    lib._chk(lib.c.tlhip_fill_u32(src.ptr, 0x3f803f80, rows * K // 2))
+    x = (r.standard_normal((70, K)).astype(np.float32).view(np.uint32) >> 16).astype(np.uint16)
+    at = np.concatenate([np.arange((1 << 18) - 30, (1 << 18) + 30), np.arange(rows - 10, rows)])
+    for ptr, a in ((src.ptr + int(at[0]) * K * 2, x[:60]), (src.ptr + int(at[60]) * K * 2, x[60:])):
+        a = np.ascontiguousarray(a)
+        lib._chk(lib.c.tlhip_memcpy_h2d(ptr, a.ctypes.data, a.nbytes))
+    lib.quantize_mxfp4(src, lib.T_BF16, codes, scales, rows, K)
+    lib.dequantize_mxfp4(codes, scales, src, lib.T_BF16, rows, K)
+    want_c, want_s = mx.quantize((x.astype(np.uint32) << 16).view(np.float32), True)
+    want = mx.values(want_c, want_s, True)
+
+    def read(b, row, each, dtype):
+        out = np.empty(each, dtype)
+        lib._chk(lib.c.tlhip_memcpy_d2h(out.ctypes.data, b.ptr + int(row) * out.nbytes, out.nbytes))
+        return out
+
+    for i, row in enumerate(at):
+        assert np.array_equal(read(codes, row, K // 2, np.uint8), mx.pack(want_c[i:i + 1])[0]), row
+        assert np.array_equal(read(scales, row, K // 32, np.uint8), want_s[i]), row
+        assert np.array_equal((read(src, row, K, np.uint16).astype(np.uint32) << 16).view(np.float32), want[i].astype(np.float32)), row
+    for row in (0, 12345, at[0] - 1, at[59] + 1 if at[59] + 1 < at[60] else 1):       # 1 = 4 x 2^-2
+        assert (read(codes, row, K // 2, np.uint8) == 0x66).all() and (read(scales, row, K // 32, np.uint8) == 125).all()
+        assert (read(src, row, K, np.uint16) == 0x3f80).all()
+    for b in (src, codes, scales):
         b.free()
