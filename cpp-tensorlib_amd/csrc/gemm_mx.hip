@@ -13,10 +13,11 @@ namespace tlhip {
 // serves together find different banks. A row's four scale bytes of a step are one word, which a lane shifts down to its own block's.
 // WORDS: that word is a whole one in memory, too (K % 128 == 0, so that no step ends past a row); elsewhere it is read
 // from wherever it lies.
-// Bound by the matrix cores: each element is multiplied twice, as its large and its small half, so their ceiling is half the
-// formats' (about 1.9e15 products and sums a second at the clock that such a load leaves). 2048 x 37888 x 3584 with the gate takes
-// 390 us (1.43e15 a second), 512 x 3584 x 18944 66 us (1.05e15, four parts' traffic and their sum in it). The activations straight
-// into registers took 484 us instead of 436; a third stage of LDS and raised wave priorities changed nothing.
+// Bound by the matrix cores where there are many tiles: each element is multiplied twice, as its large and its small half, so their
+// ceiling is half the formats' (about 1.9e15 products and sums a second at the clock that such a load leaves). 2048 x 37888 x 3584 with
+// the gate takes 390 us (1.43e15 a second), 512 x 3584 x 18944 66 us (1.05e15, four parts' traffic and their sum in it), but 512 x 4608 x
+// 3584, 2.25 tiles of 64 x 64 a CU, 27.7 (0.61e15). The activations straight into registers took 484 us instead of 436; a third stage of LDS
+// and raised wave priorities changed nothing.
 typedef uint32_t any4 __attribute__((aligned(1)));
 __device__ __forceinline__ uint32_t short_row(const uint8_t* row, int nb) {      // the scales of a row that has one to three
   uint32_t v = row[0];

@@ -132,7 +132,7 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
 // xout = x + (parts[0] + parts[1] + ...), h = xout / sqrt(mean(xout^2) + eps) * w, h as MXFP8: a block per row, a thread V times eight numbers,
 // which stay in its registers. The statistic and h are formed in 64 bits and h is rounded to f32 once: an element next to the border
 // between two codes then falls on the same side however the sum is split, so a row's bytes do not depend on the launch's shape.
-// One row of 896 4.4 us (with the row in LDS and the sum through shuffles 5.1; an empty launch is 3.3), 301 of 3584 with three parts
+// One row of 896 4.6 to 5.1 us from machine to machine (with the row in LDS and the sum through shuffles 0.7 more; an empty launch is 3.3), 301 of 3584 with three parts
 // 7.1 (a copy's rate would be 4.2 beside the launch), 2048 of 8192 with two 58, 5.0 TB/s. Sixteen numbers a thread where eight would do: 301 of 3584
 // with three parts 6.0 instead of 6.4 in a queue of launches, but 257 with two 4.8 instead of 4.5, 2048 of 8192 60 instead of 58.
 template <int V>

@@ -55,7 +55,8 @@ inline bool gemv_attn(const linear& L, void* parts, int n_parts, int64_t heads, 
 inline bool gemm(const linear& L, void* a, void* out, int64_t T) {
   if (L.fmt == wfmt::q4)
     return hip::gemm_q4_nt(a, L.w, static_cast<char*>(L.w) + L.N * L.K / 2, out, T, L.N, L.K, kQ4Group);
-  if (L.fmt == wfmt::mxfp4) {   // f32 rows meet an mxfp4 weight row by row, none of them rounded to MXFP8
+  // f32 rows meet an mxfp4 weight row by row, none of them rounded to MXFP8; each reads the weight (152064 x 3584: 52 us)
+  if (L.fmt == wfmt::mxfp4) {
     bool ok = true;
     for (int64_t t = 0; t < T && ok; t++)
       ok = gemv(L, static_cast<char*>(a) + t * L.K * 4, static_cast<char*>(out) + t * L.N * 4);
